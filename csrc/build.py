@@ -28,6 +28,10 @@ PKG = os.path.join(ROOT, "pytorch_multiprocessing_distributed_amd")
 BUILD = os.path.join(ROOT, "build", "csrc")
 ARCH = os.environ.get("PMD_OFFLOAD_ARCH", "gfx950")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
+# the packed fp32 instructions stay off in device code (-O3 forms them from scalar float code by
+# itself, and some of their forms have given wrong results now and then on this hardware); the
+# host pass does not know the feature and says so
+DEVICE_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def _torch_paths():
@@ -127,12 +131,12 @@ def build(force=False, jobs=None, debug=False, verbose=True, asan=False, variant
     inc, lib, abi = _torch_paths()
     headers = glob.glob(os.path.join(CSRC, "kernels", "*.h"))
     opt = ["-O1", "-g"] if (debug or asan) else ["-O3"]
-    common = [HIPCC, f"--offload-arch={ARCH}", "-std=c++17", "-fPIC", *opt,
+    common = [HIPCC, f"--offload-arch={ARCH}", "-std=c++17", "-fPIC", *opt, *DEVICE_FLAGS,
               "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
               *os.environ.get("PMD_EXTRA_CFLAGS", "").split()]  # A/B variant macros
     jobs_ = []
     objs = []
-    kcommon = [HIPCC, f"--offload-arch={ARCH}", "-std=c++17", "-fPIC", "-O3",
+    kcommon = [HIPCC, f"--offload-arch={ARCH}", "-std=c++17", "-fPIC", "-O3", *DEVICE_FLAGS,
                "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
                *os.environ.get("PMD_EXTRA_CFLAGS", "").split()]
     stamps = []
