@@ -770,6 +770,92 @@ std::vector<Tensor> bn_bwd_elemt(Tensor dout, c10::optional<Tensor> mask, Tensor
   return {dy};
 }
 
+// ------------------------------------------------------------ group norm
+static int act_esize(const Tensor& t, const char* what) {
+  TORCH_CHECK(t.scalar_type() == torch::kBFloat16 || t.scalar_type() == torch::kFloat32, what,
+              " must be bf16 or fp32, got ", t.scalar_type());
+  return t.scalar_type() == torch::kBFloat16 ? 2 : 4;
+}
+static void same_as(const Tensor& t, const Tensor& x, const char* what) {
+  TORCH_CHECK(t.device() == x.device() && t.scalar_type() == x.scalar_type() && t.sizes() == x.sizes() &&
+              t.is_contiguous(), what, " must be contiguous and match x in device, type and shape");
+}
+static float* channel_vec(const Tensor& t, const Tensor& x, int64_t C, const char* what) {
+  TORCH_CHECK(t.device() == x.device() && t.scalar_type() == torch::kFloat32 && t.is_contiguous() &&
+              t.numel() == C, what, " must be a contiguous fp32 [C] tensor on the device of x");
+  return t.data_ptr<float>();
+}
+static pmd::GnArgs gn_args(const Tensor& x, const c10::optional<Tensor>& res, const Tensor& gamma, const Tensor& beta,
+                           int64_t groups, double eps, int64_t act) {
+  CHECK_DEV(x); CHECK_CONT(x);
+  pmd::GnArgs a{};
+  a.esize = act_esize(x, "group_norm: x");
+  TORCH_CHECK(x.dim() >= 2, "group_norm: x must be [N, ..., C]");
+  const int64_t N = x.size(0), C = x.size(-1);
+  TORCH_CHECK(C >= 1 && C <= pmd::kGnMaxChannels, "group_norm: 1 to ", pmd::kGnMaxChannels, " channels, got ", C);
+  TORCH_CHECK(groups >= 1 && C % groups == 0, "group_norm: ", C, " channels do not split into ", groups, " groups");
+  int64_t hw = 1;
+  for (int64_t d = 1; d < x.dim() - 1; ++d) hw *= x.size(d);
+  TORCH_CHECK(N < (1ll << 25) && hw < (1ll << 31), "group_norm: too many samples or pixels");
+  TORCH_CHECK(act >= 0 && act <= 2, "group_norm: unknown activation");
+  a.N = (int)N; a.HW = (int)hw; a.C = (int)C; a.G = (int)groups; a.act = (int)act; a.eps = (float)eps;
+  a.x = x.data_ptr();
+  if (res && res->defined()) {
+    same_as(*res, x, "group_norm: residual");
+    a.res = res->data_ptr();
+  }
+  a.gamma = channel_vec(gamma, x, C, "group_norm: weight");
+  a.beta = channel_vec(beta, x, C, "group_norm: bias");
+  return a;
+}
+
+// -> (out, stats [N, G, 2])
+std::vector<Tensor> group_norm_fwd(Tensor x, c10::optional<Tensor> res, Tensor gamma, Tensor beta, int64_t groups,
+                                   double eps, int64_t act) {
+  pmd::GnArgs a = gn_args(x, res, gamma, beta, groups, eps, act);
+  c10::DeviceGuard g(x.device());
+  Tensor out = torch::empty_like(x);
+  Tensor stats = torch::empty({a.N, groups, 2}, gamma.options());
+  if (x.numel() == 0) return {out, stats};
+  Tensor ws = torch::empty({pmd::gn_fwd_workspace_floats(a.N, a.HW, a.C, a.G, a.esize)}, gamma.options());
+  a.stats = stats.data_ptr<float>();
+  a.ws = ws.data_ptr<float>();
+  a.out = out.data_ptr();
+  CHECK_RC(pmd::gn_fwd_launch(a, cur_stream()), "group_norm_fwd");
+  return {out, stats};
+}
+
+// -> (dx, dres or None); dgamma, dbeta are written (accumulate: added to)
+std::vector<Tensor> group_norm_bwd(Tensor dout, Tensor x, c10::optional<Tensor> res, Tensor gamma, Tensor beta,
+                                   Tensor stats, int64_t groups, int64_t act, Tensor dgamma, Tensor dbeta,
+                                   bool accumulate) {
+  pmd::GnArgs a = gn_args(x, res, gamma, beta, groups, 0.0, act);
+  same_as(dout, x, "group_norm: gradient");
+  TORCH_CHECK(stats.device() == x.device() && stats.scalar_type() == torch::kFloat32 && stats.is_contiguous() &&
+              stats.numel() == (int64_t)a.N * groups * 2, "group_norm: stats must be the forward's [N, G, 2]");
+  a.dgamma = channel_vec(dgamma, x, a.C, "group_norm: weight gradient");
+  a.dbeta = channel_vec(dbeta, x, a.C, "group_norm: bias gradient");
+  a.accumulate = accumulate;
+  c10::DeviceGuard g(x.device());
+  Tensor dx = torch::empty_like(x), dres;
+  if (a.res) dres = torch::empty_like(x);
+  if (x.numel() == 0) {
+    if (!accumulate) {
+      pmd::zero_launch(dgamma.data_ptr(), dgamma.nbytes(), cur_stream());
+      pmd::zero_launch(dbeta.data_ptr(), dbeta.nbytes(), cur_stream());
+    }
+    return {dx, dres};
+  }
+  Tensor ws = torch::empty({pmd::gn_bwd_workspace_floats(a.N, a.HW, a.C, a.G, a.esize)}, gamma.options());
+  a.stats = stats.data_ptr<float>();
+  a.ws = ws.data_ptr<float>();
+  a.dout = dout.data_ptr();
+  a.dx = dx.data_ptr();
+  a.dres = a.res ? dres.data_ptr() : nullptr;
+  CHECK_RC(pmd::gn_bwd_launch(a, cur_stream()), "group_norm_bwd");
+  return {dx, dres};
+}
+
 // ----------------------------------------------------------------- pools
 std::vector<Tensor> maxpool_fwd(Tensor x) {
   CHECK_DEV(x); CHECK_BF16(x); CHECK_CONT(x);
@@ -1248,6 +1334,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("gamma"), py::arg("red"), py::arg("count"), py::arg("count_h"), py::arg("relu"),
         py::arg("want_dzm"), py::arg("eval_mode"), py::arg("q8_scale") = py::none(),
         py::arg("q8_amax") = py::none(), py::arg("q8_only") = false);
+  m.def("group_norm_fwd", &group_norm_fwd);
+  m.def("group_norm_bwd", &group_norm_bwd);
   m.def("maxpool_fwd", &maxpool_fwd);
   m.def("maxpool_bwd", &maxpool_bwd);
   m.def("stem_pool_fwd", &stem_pool_fwd);

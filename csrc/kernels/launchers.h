@@ -170,6 +170,27 @@ int xent_fwd_launch(const float* logits, const long long* target, float* loss, f
                     long long* correct, int N, int V, hipStream_t st);
 int xent_bwd_launch(const float* logits, const long long* target, const float* lse, const float* gloss,
                     float* grad, int N, int V, hipStream_t st);
+// group normalisation + residual + activation, channels last (kernels/group_norm.hip)
+constexpr int kGnMaxChannels = 16384;  // two fp32 values per channel in the 160 KiB of LDS
+struct GnArgs {
+  int esize;             // 2: bf16, 4: fp32 (x, res, out, dout, dx, dres)
+  int N, HW, C, G, act;  // act: 0 none, 1 relu, 2 silu
+  float eps;
+  const void *x, *res;   // res nullable
+  const float *gamma, *beta;
+  float* stats;          // [N][G][2] mean, rstd: written by the forward, read by the backward
+  float* ws;             // gn_*_workspace_floats
+  void* out;             // forward
+  const void* dout;      // backward
+  void *dx, *dres;       // dres with res
+  float *dgamma, *dbeta;
+  bool accumulate;       // dgamma, dbeta += (gradient-arena targets)
+};
+long long gn_fwd_workspace_floats(int N, int HW, int C, int G, int esize);
+long long gn_bwd_workspace_floats(int N, int HW, int C, int G, int esize);
+int gn_fwd_launch(const GnArgs& a, hipStream_t st);
+int gn_bwd_launch(const GnArgs& a, hipStream_t st);
+
 int zero_launch(void* ptr, long long nbytes, hipStream_t st);  // memset 0 (framework kernel)
 int sgd_launch(float* p, const float* g, float* buf, long long n, float lr, const float* lr_dev,
                float momentum, float wd, float damp, bool nesterov, bool first, hipStream_t st);

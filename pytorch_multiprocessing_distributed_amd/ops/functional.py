@@ -38,6 +38,7 @@ import os
 import weakref
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import torch_prims
 
@@ -1511,6 +1512,75 @@ def residual_block(x, stages, final, shortcut, training):
     """Run a ResNet block (see :class:`_ResidualBlockFn`) as one autograd node."""
     cfg = (tuple(stages), final, shortcut, training)
     return _ResidualBlockFn.apply(cfg, x, *_block_params(stages, final, shortcut))
+
+
+# ---------------------------------------------------------------- group norm
+def _param_grads(needs, ps, write):
+    """Gradients of the parameters ``ps`` by ``write(targets, accumulate)``: added to their arena
+    views when all live there (then reported ready, and None is returned for each), else written to
+    new fp32 tensors."""
+    tg = [_grad_target(p) for p in ps]
+    if all(t is not None for t in tg):
+        write(tg, True)
+        _ready(*ps)
+        return [None] * len(ps)
+    out = [torch.empty_like(p, dtype=p.dtype if p.dtype == torch.float64 else torch.float32) for p in ps]
+    write(out, False)
+    return [o.to(p.dtype) if n else None for o, p, n in zip(out, ps, needs)]
+
+
+class _GroupNormActFn(torch.autograd.Function):
+    """out = act( GN(x) + res ), one node; saves x (and res) and the [N, G] statistics, and the
+    backward takes the activation's slope from them again."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, res, groups, eps, act):
+        P = prims_for(x)
+        out, stats = P.group_norm_fwd(x, res, weight, bias, groups, eps, act)
+        ctx.save_for_backward(x, res, weight, bias, stats)
+        ctx.params = (weight, bias)
+        ctx.cfg = (groups, act)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        x, res, weight, bias, stats = ctx.saved_tensors
+        groups, act = ctx.cfg
+        P = prims_for(x)
+        r = []
+
+        def write(tgt, accumulate):
+            r.extend(P.group_norm_bwd(dout.contiguous(), x, res, weight, bias, stats, groups, act,
+                                      tgt[0], tgt[1], accumulate))
+        dw, db = _param_grads(ctx.needs_input_grad[1:3], ctx.params, write)
+        return r[0], dw, db, r[1] if ctx.needs_input_grad[3] else None, None, None, None
+
+
+def group_norm_act(x, gn, residual=None, act="relu"):
+    """``act(GroupNorm(x) + residual)`` of a channels-last activation in one pass forward and one
+    backward node: the norm beside :func:`bn_add_act` for batches too small for batch statistics
+    (no exchange between ranks, no running statistics; training and evaluation are the same).
+
+    ``x`` [N, ..., C] (bf16 or fp32), ``gn`` a module with ``num_groups``, ``eps`` and fp32 ``weight``
+    / ``bias`` of C values (``torch.nn.GroupNorm``), ``residual`` like ``x`` or None, ``act`` one of
+    "none", "relu", "silu".  Statistics, sums and the activation are computed in fp32.  Tensors that
+    are not contiguous are laid out first.  On a GPU C is at most 16,384."""
+    if act not in torch_prims.GN_ACTS:
+        raise ValueError(f"unknown activation {act!r}; choose from {torch_prims.GN_ACTS}")
+    if gn.weight is None or gn.bias is None:
+        raise ValueError("group_norm_act needs a GroupNorm with weight and bias")
+    if x.dim() < 2 or x.shape[-1] != gn.weight.numel():
+        raise ValueError(f"x must be [N, ..., {gn.weight.numel()}], got {tuple(x.shape)}")
+    if x.shape[-1] % gn.num_groups:
+        raise ValueError(f"{x.shape[-1]} channels do not split into {gn.num_groups} groups")
+    if residual is not None:
+        if residual.shape != x.shape or residual.dtype != x.dtype:
+            raise ValueError(f"residual must be {tuple(x.shape)} {x.dtype}, got "
+                             f"{tuple(residual.shape)} {residual.dtype}")
+        residual = residual.contiguous()
+    return _GroupNormActFn.apply(x.contiguous(), gn.weight, gn.bias, residual, int(gn.num_groups),
+                                 float(gn.eps), act)
 
 
 # --------------------------------------------------------------------- pools

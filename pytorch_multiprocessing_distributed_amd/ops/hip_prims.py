@@ -210,6 +210,19 @@ def bn_bwd_elemt_eval(dout, mask, p, relu, want_dzm=False):
     return (r[0], r[1]) if want_dzm else (r[0], None)
 
 
+# --------------------------------------------------------------- group norm
+def group_norm_fwd(x, res, gamma, beta, groups, eps, act):
+    """-> (act(GN(x) + res), stats [N, G, 2] = mean, rstd)."""
+    return tuple(_C.group_norm_fwd(x, res, gamma.detach(), beta.detach(), int(groups), float(eps),
+                                   _TP.GN_ACTS.index(act)))
+
+
+def group_norm_bwd(dout, x, res, gamma, beta, stats, groups, act, dgamma, dbeta, accumulate):
+    """-> (dx, dres or None); dgamma, dbeta (fp32 [C]) are written, or added to."""
+    return tuple(_C.group_norm_bwd(dout, x, res, gamma.detach(), beta.detach(), stats, int(groups),
+                                   _TP.GN_ACTS.index(act), dgamma, dbeta, bool(accumulate)))
+
+
 # -------------------------------------------------------------------- pools
 def maxpool_fwd(x):
     out, arg = _C.maxpool_fwd(x)

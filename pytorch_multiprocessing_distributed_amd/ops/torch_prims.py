@@ -247,6 +247,58 @@ def bn_bwd_elemt_eval(dout, mask, p, relu, want_dzm=False):
     return dy, (d.to(dout.dtype) if want_dzm else None)
 
 
+# --------------------------------------------------------------- group norm
+GN_ACTS = ("none", "relu", "silu")
+
+
+def _gn_z(x, res, gamma, beta, stats, groups):
+    """(xhat, z) as [N, pixels, G, C/G] in the accumulation dtype."""
+    n, c = x.shape[0], x.shape[-1]
+    xf = _f(x).reshape(n, -1, groups, c // groups) if x.numel() else _f(x).reshape(n, 0, groups, c // groups)
+    xhat = (xf - stats[:, None, :, :1]) * stats[:, None, :, 1:]
+    z = xhat * _f(gamma.detach()).reshape(groups, -1) + _f(beta.detach()).reshape(groups, -1)
+    if res is not None:
+        z = z + _f(res).reshape(z.shape)
+    return xhat, z
+
+
+def group_norm_fwd(x, res, gamma, beta, groups, eps, act):
+    """-> (act(GN(x) + res), stats [N, G, 2] = mean, rstd) of a channels-last x."""
+    n, c = x.shape[0], x.shape[-1]
+    if x.numel() == 0:
+        return torch.empty_like(x), torch.zeros(n, groups, 2, dtype=_f(x).dtype, device=x.device)
+    xf = _f(x).reshape(n, -1, groups, c // groups)
+    var, mean = torch.var_mean(xf, dim=(1, 3), unbiased=False)
+    stats = torch.stack([mean, torch.rsqrt(var + eps)], dim=-1)
+    _, z = _gn_z(x, res, gamma, beta, stats, groups)
+    if act == "relu":
+        z = z.clamp_min(0.0)
+    elif act == "silu":
+        z = z * torch.sigmoid(z)
+    return z.reshape(x.shape).to(x.dtype), stats
+
+
+def group_norm_bwd(dout, x, res, gamma, beta, stats, groups, act, dgamma, dbeta, accumulate):
+    """-> (dx, dres or None); dgamma, dbeta are written, or added to."""
+    xhat, z = _gn_z(x, res, gamma, beta, stats, groups)
+    dz = _f(dout).reshape(z.shape)
+    if act == "relu":
+        dz = torch.where(z <= 0, torch.zeros_like(dz), dz)
+    elif act == "silu":
+        s = torch.sigmoid(z)
+        dz = dz * (s * (1.0 + z * (1.0 - s)))
+    dg, db = (dz * xhat).sum(dim=(0, 1)).reshape(-1), dz.sum(dim=(0, 1)).reshape(-1)
+    for tgt, g in ((dgamma, dg), (dbeta, db)):
+        if accumulate:
+            tgt.add_(g.to(tgt.dtype))
+        else:
+            tgt.copy_(g)
+    dh = dz * _f(gamma.detach()).reshape(groups, -1)
+    dx = dh - dh.mean(dim=(1, 3), keepdim=True) - xhat * (dh * xhat).mean(dim=(1, 3), keepdim=True)
+    dx = (dx * stats[:, None, :, 1:]).reshape(x.shape).to(x.dtype)
+    return dx, (dz.reshape(x.shape).to(x.dtype) if res is not None else None)
+
+
 # -------------------------------------------------------------------- pools
 def maxpool_fwd(x):
     """3x3/s2/p1 max-pool; the auxiliary output is the input itself (the
