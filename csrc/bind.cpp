@@ -856,6 +856,105 @@ std::vector<Tensor> group_norm_bwd(Tensor dout, Tensor x, c10::optional<Tensor> 
   return {dx, dres};
 }
 
+// ------------------------------------------------- linear cross-entropy
+static pmd::LxShape lx_shape(const Tensor& x, const Tensor& w, const c10::optional<Tensor>& b, const Tensor& target,
+                             bool bf16_products, pmd::LxIo& io) {
+  CHECK_DEV(x); CHECK_CONT(x); CHECK_CONT(w); CHECK_CONT(target);
+  const bool x16 = act_esize(x, "linear_xent: x") == 2, w16 = act_esize(w, "linear_xent: weight") == 2;
+  TORCH_CHECK(x.dim() == 2 && w.dim() == 2 && x.size(1) == w.size(1), "linear_xent: x [N, D], weight [V, D]");
+  TORCH_CHECK(w.device() == x.device() && target.device() == x.device(),
+              "linear_xent: x, weight and target must be on one device");
+  TORCH_CHECK(target.scalar_type() == torch::kInt64 && target.dim() == 1 && target.size(0) == x.size(0),
+              "linear_xent: target must be int64 [N]");
+  TORCH_CHECK(x.size(0) <= (1 << 24) && w.size(0) >= 1 && w.size(0) <= (1 << 30) && x.size(1) >= 1 &&
+              x.size(1) <= (1 << 21) - 8, "linear_xent: at most 2^24 rows, 2^30 classes, 2^21 - 8 features");
+  pmd::LxShape s{};
+  s.N = (int)x.size(0); s.V = (int)w.size(0); s.D = (int)x.size(1);
+  s.planes = bf16_products || (x16 && w16) ? 1 : 3;
+  s.x_f32 = !x16; s.w_f32 = !w16;
+  s.w_aligned = reinterpret_cast<uintptr_t>(w.data_ptr()) % 16 == 0;
+  io.x = x.data_ptr(); io.w = w.data_ptr();
+  io.target = reinterpret_cast<const long long*>(target.data_ptr<int64_t>());
+  if (b && b->defined()) {
+    s.b_f32 = act_esize(*b, "linear_xent: bias") == 4;
+    TORCH_CHECK(b->device() == x.device() && b->is_contiguous() && b->numel() == s.V,
+                "linear_xent: bias must be [V] on the device of x");
+    io.bias = b->data_ptr();
+  }
+  return s;
+}
+
+// -> (loss [1], correct [1], lse [N], inv_count [1])
+std::vector<Tensor> linear_xent_fwd(Tensor x, Tensor w, c10::optional<Tensor> b, Tensor target, int64_t ignore,
+                                    bool bf16_products) {
+  pmd::LxIo io{};
+  const pmd::LxShape s = lx_shape(x, w, b, target, bf16_products, io);
+  c10::DeviceGuard g(x.device());
+  auto f32 = x.options().dtype(torch::kFloat32);
+  Tensor loss = torch::empty({1}, f32), lse = torch::empty({s.N}, f32), inv = torch::empty({1}, f32);
+  Tensor correct = torch::empty({1}, x.options().dtype(torch::kInt64));
+  if (s.N == 0) {
+    pmd::zero_launch(loss.data_ptr(), loss.nbytes(), cur_stream());
+    pmd::zero_launch(correct.data_ptr(), correct.nbytes(), cur_stream());
+    return {loss, correct, lse, inv};
+  }
+  Tensor ws = torch::empty({pmd::lx_workspace_bytes(s, false)}, x.options().dtype(torch::kUInt8));
+  io.ignore = ignore;
+  io.ws = ws.data_ptr();
+  io.loss = loss.data_ptr<float>();
+  io.lse = lse.data_ptr<float>();
+  io.inv_count = inv.data_ptr<float>();
+  io.correct = reinterpret_cast<long long*>(correct.data_ptr<int64_t>());
+  CHECK_RC(pmd::lx_fwd_launch(s, io, cur_stream()), "linear_xent_fwd");
+  return {loss, correct, lse, inv};
+}
+
+// -> dx (None unless want_dx); dw, db are written, or added to (fp32)
+Tensor linear_xent_bwd(Tensor gloss, Tensor x, Tensor w, c10::optional<Tensor> b, Tensor target, int64_t ignore,
+                       bool bf16_products, Tensor lse, Tensor inv_count, bool want_dx, c10::optional<Tensor> dw,
+                       c10::optional<Tensor> db, bool accumulate) {
+  pmd::LxIo io{};
+  const pmd::LxShape s = lx_shape(x, w, b, target, bf16_products, io);
+  CHECK_F32(gloss); CHECK_F32(lse); CHECK_F32(inv_count); CHECK_CONT(lse);
+  TORCH_CHECK(gloss.device() == x.device() && lse.device() == x.device() && inv_count.device() == x.device() &&
+              gloss.numel() == 1 && inv_count.numel() == 1 && lse.numel() == s.N, "linear_xent: saved tensors");
+  c10::DeviceGuard g(x.device());
+  Tensor dx;
+  if (want_dx) {
+    dx = torch::empty_like(x);
+    io.dx = dx.data_ptr();
+  }
+  if (dw && dw->defined()) {
+    TORCH_CHECK(dw->device() == x.device() && dw->sizes() == w.sizes() && dw->is_contiguous() &&
+                (dw->scalar_type() == torch::kFloat32 || (dw->scalar_type() == torch::kBFloat16 && !accumulate)),
+                "linear_xent: weight gradient must be [V, D] like the weight (fp32 to accumulate)");
+    io.dw = dw->data_ptr();
+    io.dw_f32 = dw->scalar_type() == torch::kFloat32;
+  }
+  if (db && db->defined()) {
+    TORCH_CHECK(io.bias && db->device() == x.device() && db->numel() == s.V && db->is_contiguous() &&
+                db->scalar_type() == b->scalar_type() && (s.b_f32 || !accumulate),
+                "linear_xent: bias gradient must be [V] like the bias (fp32 to accumulate)");
+    io.db = db->data_ptr();
+  }
+  if (s.N == 0) {
+    if (!accumulate) {
+      if (io.dw) pmd::zero_launch(io.dw, dw->nbytes(), cur_stream());
+      if (io.db) pmd::zero_launch(io.db, db->nbytes(), cur_stream());
+    }
+    return dx;
+  }
+  Tensor ws = torch::empty({pmd::lx_workspace_bytes(s, true)}, x.options().dtype(torch::kUInt8));
+  io.ignore = ignore;
+  io.ws = ws.data_ptr();
+  io.lse = lse.data_ptr<float>();
+  io.inv_count = inv_count.data_ptr<float>();
+  io.gloss = gloss.data_ptr<float>();
+  io.accumulate = accumulate;
+  CHECK_RC(pmd::lx_bwd_launch(s, io, cur_stream()), "linear_xent_bwd");
+  return dx;
+}
+
 // ----------------------------------------------------------------- pools
 std::vector<Tensor> maxpool_fwd(Tensor x) {
   CHECK_DEV(x); CHECK_BF16(x); CHECK_CONT(x);
@@ -1336,6 +1435,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("q8_amax") = py::none(), py::arg("q8_only") = false);
   m.def("group_norm_fwd", &group_norm_fwd);
   m.def("group_norm_bwd", &group_norm_bwd);
+  m.def("linear_xent_fwd", &linear_xent_fwd);
+  m.def("linear_xent_bwd", &linear_xent_bwd);
   m.def("maxpool_fwd", &maxpool_fwd);
   m.def("maxpool_bwd", &maxpool_bwd);
   m.def("stem_pool_fwd", &stem_pool_fwd);

@@ -191,6 +191,28 @@ long long gn_bwd_workspace_floats(int N, int HW, int C, int G, int esize);
 int gn_fwd_launch(const GnArgs& a, hipStream_t st);
 int gn_bwd_launch(const GnArgs& a, hipStream_t st);
 
+// softmax cross-entropy of a linear classifier without its logits (kernels/linear_xent.hip)
+struct LxShape {
+  int N, V, D;
+  int planes;                        // 1: bf16 products, 3: fp32 operands as three bf16 planes
+  bool x_f32, w_f32, b_f32;          // else bf16
+  bool w_aligned;                    // 16-byte aligned weight rows
+};
+struct LxIo {
+  const void *x, *w, *bias;          // [N][D], [V][D], [V] or nullptr
+  const long long* target;           // [N]
+  long long ignore;
+  void* ws;                          // lx_workspace_bytes
+  float *loss, *lse, *inv_count;     // [1], [N], [1]; lse and inv_count are the backward's inputs
+  long long* correct;                // [1]
+  const float* gloss;                // backward: d(loss) [1]
+  void *dx, *dw, *db;                // nullable; dx in x's type, db in the bias's
+  bool dw_f32, accumulate;           // accumulate: dw, db (fp32) +=
+};
+long long lx_workspace_bytes(const LxShape& s, bool bwd);
+int lx_fwd_launch(const LxShape& s, const LxIo& io, hipStream_t st);
+int lx_bwd_launch(const LxShape& s, const LxIo& io, hipStream_t st);
+
 int zero_launch(void* ptr, long long nbytes, hipStream_t st);  // memset 0 (framework kernel)
 int sgd_launch(float* p, const float* g, float* buf, long long n, float lr, const float* lr_dev,
                float momentum, float wd, float damp, bool nesterov, bool first, hipStream_t st);

@@ -1,0 +1,694 @@
+// Softmax cross-entropy of a linear classifier, straight from the features (gfx950).
+//
+//   l = x W^T + b   x [N][D], W [V][D]      loss = sum_{rows kept} (lse(l_i) - l_i[t_i]) / max(kept, 1)
+//   dl = (softmax(l) - onehot(t)) gloss / kept   (rows kept; zero elsewhere)
+//   dx = dl W,  dW = dl^T x,  db = column sums of dl
+//
+// The logits are never stored.  Forward: the product's epilogue reduces its tile to (max, sum of
+// exponentials, argmax) per row, one combine pass joins the column tiles, one block sums the rows.
+// Backward, per piece of the vocabulary: the piece's logits are computed again and their epilogue
+// writes softmax - onehot in 16 bits (a piece holds at most kPieceBytes, which the last-level cache
+// keeps); the two gradient products read it from there.  That is 8 N V D operations where keeping
+// the logits would need 6.
+//
+// Rounding: operands are bf16 (products are then exact in fp32), or fp32 held as three bf16 planes
+// (gemm_core.h).  softmax - onehot is rounded to the same: one bf16 when the operands are bf16 --
+// half a bf16 step of each probability, the size of the gradients' own rounding -- or three planes.
+// Sums, statistics, the loss and db stay in fp32 (db sums the probabilities before that rounding).
+// No atomics: partial results are joined in a fixed order.
+//
+// Rows whose target is ignore_index count for nothing whatever they hold (their features are
+// replaced by zeros before the product).  A target outside [0, V) makes the row's loss NaN.
+#include "gemm_core.h"
+
+namespace pmd {
+
+namespace {
+
+constexpr long long kPieceBytes = 192ll << 20;
+
+__device__ __forceinline__ float ld_any(const void* p, long long i, bool f32) {
+  return f32 ? static_cast<const float*>(p)[i] : bf2f(static_cast<const bf16_t*>(p)[i]);
+}
+
+// v as a sum of PL bf16 (each the rounding of what the ones before it leave)
+template <int PL>
+__device__ __forceinline__ void to_planes(float v, bf16_t (&o)[PL]) {
+#pragma unroll
+  for (int p = 0; p < PL; ++p) {
+    o[p] = f2bf(v);
+    v -= bf2f(o[p]);
+  }
+}
+
+// src [rows][cols] (bf16 or fp32, row stride lds) -> PL planes [rows][ld], zero-padded columns; with
+// target: rows to ignore become zero
+template <int PL>
+__global__ __launch_bounds__(256) void lx_prep_kernel(const void* __restrict__ src, int f32, long long lds, int rows,
+                                                      int cols, bf16_t* __restrict__ dst, long long plane, int ld,
+                                                      const long long* __restrict__ target, long long ignore) {
+  const int c8 = ld >> 3;
+  const long long total = (long long)rows * c8;
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+    const int r = (int)(i / c8), c = (int)(i - (long long)r * c8) * 8;
+    const bool skip = target && target[r] == ignore;
+    bf16_t o[8][PL];
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      to_planes<PL>(!skip && c + k < cols ? ld_any(src, r * lds + c + k, f32) : 0.f, o[k]);
+#pragma unroll
+    for (int p = 0; p < PL; ++p) {
+      uint32_t w[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) w[k] = (uint32_t)o[2 * k][p] | ((uint32_t)o[2 * k + 1][p] << 16);
+      *reinterpret_cast<uint4*>(dst + p * plane + (long long)r * ld + c) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+}
+
+template <int PL>
+struct LxArgs {
+  GemmOperand<PL> x, w;  // rows N x D, V x D (w from the piece's first row in the backward)
+  int N, V, D;           // V: classes (of the piece)
+  const void* bias;      // nullable, from the piece's first class
+  int bias_f32;
+  const long long* target;
+  long long ignore;
+  int v0;                // first class of the piece
+  // forward
+  float *pmax, *psum;    // [column tiles][N]
+  int* pidx;
+  float* tlogit;         // [N]
+  // backward
+  const float* lse;      // [N]
+  bf16_t* prob;          // PL planes [N][ldp]
+  long long pplane;
+  int ldp;
+  float* dbpart;         // [row tiles][ldp], nullable
+};
+
+__device__ __forceinline__ float bias_of(const void* bias, int f32, int n, int V) {
+  return bias && n < V ? ld_any(bias, n, f32) : 0.f;
+}
+
+// ---------------------------------------------------------------- forward
+template <class G>
+__global__ __launch_bounds__(G::NT) void lx_fwd_kernel(LxArgs<G::PL> a) {
+  __shared__ __attribute__((aligned(16))) char smem[G::LDS];
+  const int tm = (a.N + G::BM - 1) / G::BM, tn = (a.V + G::BN - 1) / G::BN;
+  int im, in;
+  tile_of(blockIdx.x, tm * tn, tm, tn, im, in);
+  const int m0 = im * G::BM, n0 = in * G::BN;
+  typename G::Acc acc;
+  G::run(a.x, a.w, m0, n0, 0, a.D, smem, acc);
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, wm = wid / G::WN, wn = wid % G::WN;
+  const int nb = n0 + wn * G::TN + (lane >> 4) * 4;
+  float bias[G::NI][4];
+#pragma unroll
+  for (int j = 0; j < G::NI; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) bias[j][e] = bias_of(a.bias, a.bias_f32, nb + j * 16 + e, a.V);
+  float* sm = reinterpret_cast<float*>(smem);  // [WN][BM] max, sum, index
+  float* ss = sm + G::WN * G::BM;
+  int* si = reinterpret_cast<int*>(ss + G::WN * G::BM);
+#pragma unroll
+  for (int i = 0; i < G::MI; ++i) {
+    const int ml = wm * G::TM + i * 16 + (lane & 15), m = m0 + ml;
+    const long long t = m < a.N ? a.target[m] : -1;
+    float mx = -INFINITY;
+    int mi = 0x7fffffff;
+#pragma unroll
+    for (int j = 0; j < G::NI; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int n = nb + j * 16 + e;
+        float v = acc[i][j][e] + bias[j][e];
+        if (n >= a.V) v = -INFINITY;
+        acc[i][j][e] = v;
+        if (v > mx) {
+          mx = v;
+          mi = n;
+        }
+        if (n == t && n < a.V) a.tlogit[m] = v;
+      }
+#pragma unroll
+    for (int o = 16; o <= 32; o <<= 1) {
+      const float om = __shfl_xor(mx, o, 64);
+      const int oi = __shfl_xor(mi, o, 64);
+      if (om > mx || (om == mx && oi < mi)) {
+        mx = om;
+        mi = oi;
+      }
+    }
+    const float ref = mx == -INFINITY ? 0.f : mx;  // nothing above -inf: the sum is 0, not NaN
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < G::NI; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s += __expf(acc[i][j][e] - ref);
+    s += __shfl_xor(s, 16, 64);
+    s += __shfl_xor(s, 32, 64);
+    if (lane < 16) {
+      sm[wn * G::BM + ml] = mx;
+      ss[wn * G::BM + ml] = s;
+      si[wn * G::BM + ml] = mi;
+    }
+  }
+  __syncthreads();
+  for (int r = tid; r < G::BM; r += G::NT) {
+    if (m0 + r >= a.N) continue;
+    float mx = sm[r];
+    int mi = si[r];
+#pragma unroll
+    for (int q = 1; q < G::WN; ++q)
+      if (sm[q * G::BM + r] > mx) {  // a tie stays with the lower columns
+        mx = sm[q * G::BM + r];
+        mi = si[q * G::BM + r];
+      }
+    const float ref = mx == -INFINITY ? 0.f : mx;
+    float s = 0.f;
+#pragma unroll
+    for (int q = 0; q < G::WN; ++q) s += ss[q * G::BM + r] * __expf((sm[q * G::BM + r] == -INFINITY ? ref : sm[q * G::BM + r]) - ref);
+    const long long o = (long long)in * a.N + m0 + r;
+    a.pmax[o] = mx;
+    a.psum[o] = s;
+    a.pidx[o] = mi;
+  }
+}
+
+// joins the column tiles of 16 rows a block: lse [N], row loss [N] (0 for rows to ignore), hit [N]
+// (1: kept, 2: kept and top-1 right)
+__global__ __launch_bounds__(256) void lx_combine_kernel(const float* __restrict__ pmax, const float* __restrict__ psum,
+                                                         const int* __restrict__ pidx, const float* __restrict__ tlogit,
+                                                         const long long* __restrict__ target, long long ignore, int N,
+                                                         int V, int tiles, float* __restrict__ lse,
+                                                         float* __restrict__ rloss, int* __restrict__ hit) {
+  __shared__ float sm[16][17], ss[16][17];
+  __shared__ int si[16][17];
+  const int r = threadIdx.x & 15, q = threadIdx.x >> 4, m = blockIdx.x * 16 + r;
+  float mx = -INFINITY, s = 0.f;
+  int mi = 0x7fffffff;
+  if (m < N)
+    for (int t = q; t < tiles; t += 16) {
+      const long long o = (long long)t * N + m;
+      const float om = pmax[o], os = psum[o];
+      const int oi = pidx[o];
+      if (om > mx || (om == mx && oi < mi)) {
+        s = (mx == om ? s : s * __expf(mx - om)) + os;  // equal: both may be -inf
+        mx = om;
+        mi = oi;
+      } else {
+        s += mx == om ? os : os * __expf(om - mx);
+      }
+    }
+  sm[q][r] = mx;
+  ss[q][r] = s;
+  si[q][r] = mi;
+  __syncthreads();
+  if (q == 0 && m < N) {
+    for (int k = 1; k < 16; ++k)
+      if (sm[k][r] > mx || (sm[k][r] == mx && si[k][r] < mi)) {
+        mx = sm[k][r];
+        mi = si[k][r];
+      }
+    const float ref = mx == -INFINITY ? 0.f : mx;
+    s = 0.f;
+    for (int k = 0; k < 16; ++k) s += sm[k][r] == -INFINITY ? ss[k][r] : ss[k][r] * __expf(sm[k][r] - ref);
+    const long long t = target[m];
+    const bool keep = t != ignore, in = t >= 0 && t < V;
+    const float l = mx + __logf(s);
+    lse[m] = keep && !in ? NAN : l;
+    rloss[m] = !keep ? 0.f : in ? l - tlogit[m] : NAN;
+    hit[m] = !keep ? 0 : (t == mi ? 2 : 1);
+  }
+}
+
+// loss = sum of the row losses / kept, correct, 1 / kept
+__global__ __launch_bounds__(1024) void lx_loss_kernel(const float* __restrict__ rloss, const int* __restrict__ hit,
+                                                       int N, float* __restrict__ loss, long long* __restrict__ correct,
+                                                       float* __restrict__ inv_count) {
+  __shared__ float sl[16];
+  __shared__ int sk[16], sc[16];
+  float l = 0.f;
+  int k = 0, c = 0;
+  for (int i = threadIdx.x; i < N; i += 1024) {
+    l += rloss[i];
+    k += hit[i] > 0;
+    c += hit[i] == 2;
+  }
+  for (int o = 32; o > 0; o >>= 1) {
+    l += __shfl_xor(l, o, 64);
+    k += __shfl_xor(k, o, 64);
+    c += __shfl_xor(c, o, 64);
+  }
+  if ((threadIdx.x & 63) == 0) {
+    sl[threadIdx.x >> 6] = l;
+    sk[threadIdx.x >> 6] = k;
+    sc[threadIdx.x >> 6] = c;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 16; ++w) {
+      l += sl[w];
+      k += sk[w];
+      c += sc[w];
+    }
+    const float n = k > 0 ? (float)k : 1.f;
+    loss[0] = l / n;
+    correct[0] = c;
+    inv_count[0] = 1.f / n;
+  }
+}
+
+// --------------------------------------------------------------- backward
+// prob = softmax - onehot of the piece (rows to ignore: 0; columns past V: 0), dbpart = its column
+// sums over the row tile
+template <class G>
+__global__ __launch_bounds__(G::NT) void lx_prob_kernel(LxArgs<G::PL> a) {
+  __shared__ __attribute__((aligned(16))) char smem[G::LDS];
+  const int tm = (a.N + G::BM - 1) / G::BM, tn = (a.ldp + G::BN - 1) / G::BN;
+  int im, in;
+  tile_of(blockIdx.x, tm * tn, tm, tn, im, in);
+  const int m0 = im * G::BM, n0 = in * G::BN;
+  typename G::Acc acc;
+  G::run(a.x, a.w, m0, n0, 0, a.D, smem, acc);
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, wm = wid / G::WN, wn = wid % G::WN;
+  const int nb = n0 + wn * G::TN + (lane >> 4) * 4;
+  float bias[G::NI][4], col[G::NI][4];
+#pragma unroll
+  for (int j = 0; j < G::NI; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      bias[j][e] = bias_of(a.bias, a.bias_f32, nb + j * 16 + e, a.V);
+      col[j][e] = 0.f;
+    }
+#pragma unroll
+  for (int i = 0; i < G::MI; ++i) {
+    const int m = m0 + wm * G::TM + i * 16 + (lane & 15);
+    if (m >= a.N) continue;
+    const long long t = a.target[m];
+    const bool keep = t != a.ignore;
+    const float lse = a.lse[m];
+#pragma unroll
+    for (int j = 0; j < G::NI; ++j) {
+      const int n = nb + j * 16;
+      if (n >= a.ldp) continue;
+      bf16_t o[4][G::PL];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float p = 0.f;
+        if (keep && n + e < a.V) {
+          p = __expf(acc[i][j][e] + bias[j][e] - lse);
+          if (t == a.v0 + n + e) p -= 1.f;
+        }
+        col[j][e] += p;
+        to_planes<G::PL>(p, o[e]);
+      }
+#pragma unroll
+      for (int q = 0; q < G::PL; ++q) {
+        const uint2 w = make_uint2((uint32_t)o[0][q] | ((uint32_t)o[1][q] << 16),
+                                   (uint32_t)o[2][q] | ((uint32_t)o[3][q] << 16));
+        *reinterpret_cast<uint2*>(a.prob + q * a.pplane + (long long)m * a.ldp + n) = w;
+      }
+    }
+  }
+  if (a.dbpart) {
+    float* sc = reinterpret_cast<float*>(smem);  // [WM][BN]
+#pragma unroll
+    for (int j = 0; j < G::NI; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float v = col[j][e];
+        for (int o = 1; o < 16; o <<= 1) v += __shfl_xor(v, o, 64);
+        if ((lane & 15) == 0) sc[wm * G::BN + wn * G::TN + j * 16 + (lane >> 4) * 4 + e] = v;
+      }
+    __syncthreads();
+    for (int c = tid; c < G::BN; c += G::NT)
+      if (n0 + c < a.ldp) {
+        float v = 0.f;
+#pragma unroll
+        for (int q = 0; q < G::WM; ++q) v += sc[q * G::BN + c];
+        a.dbpart[(long long)im * a.ldp + n0 + c] = v;
+      }
+  }
+}
+
+__device__ __forceinline__ void st4(void* p, bool f32, long long o, const float (&v)[4], int n, bool acc) {
+  if (f32) {
+    float* d = static_cast<float*>(p) + o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < n) d[e] = acc ? d[e] + v[e] : v[e];
+  } else {
+    bf16_t* d = static_cast<bf16_t*>(p) + o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < n) d[e] = f2bf(v[e]);
+  }
+}
+
+// a gradient product: dst [M][N] = or += scale * A B^T.  ws: split z of the reduction adds to slab z
+// ([splits][M][N] fp32, unscaled) instead.
+template <int PL>
+struct LxGradArgs {
+  GemmOperand<PL> A, B;
+  int M, N, K, ksplit;        // ksplit: reduction elements of a split
+  float* slab;                // nullable
+  int slab_add;               // slabs hold earlier pieces
+  void* dst;
+  long long ldd;
+  int dst_f32, accumulate;
+  const float *gloss, *inv_count;
+};
+
+template <class G>
+__global__ __launch_bounds__(G::NT) void lx_grad_kernel(LxGradArgs<G::PL> a) {
+  __shared__ __attribute__((aligned(16))) char smem[G::LDS];
+  const int tm = (a.M + G::BM - 1) / G::BM, tn = (a.N + G::BN - 1) / G::BN;
+  int im, in;
+  tile_of(blockIdx.x, tm * tn, tm, tn, im, in);
+  const int m0 = im * G::BM, n0 = in * G::BN;
+  const int k0 = blockIdx.y * a.ksplit, k1 = min(a.K, k0 + a.ksplit);
+  typename G::Acc acc;
+  G::run(a.A, a.B, m0, n0, k0, k1, smem, acc);
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, wm = wid / G::WN, wn = wid % G::WN;
+  const float sc = a.slab ? 1.f : a.gloss[0] * a.inv_count[0];
+#pragma unroll
+  for (int i = 0; i < G::MI; ++i) {
+    const int m = m0 + wm * G::TM + i * 16 + (lane & 15);
+    if (m >= a.M) continue;
+#pragma unroll
+    for (int j = 0; j < G::NI; ++j) {
+      const int n = n0 + wn * G::TN + j * 16 + (lane >> 4) * 4;
+      if (n >= a.N) continue;
+      if (a.slab) {
+        float* d = a.slab + ((long long)blockIdx.y * a.M + m) * a.N + n;  // N % 8 == 0: whole float4
+        float4 v = make_float4(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]);
+        if (a.slab_add) {
+          const float4 o = *reinterpret_cast<const float4*>(d);
+          v = make_float4(v.x + o.x, v.y + o.y, v.z + o.z, v.w + o.w);
+        }
+        *reinterpret_cast<float4*>(d) = v;
+      } else {
+        const float v[4] = {acc[i][j][0] * sc, acc[i][j][1] * sc, acc[i][j][2] * sc, acc[i][j][3] * sc};
+        st4(a.dst, a.dst_f32, (long long)m * a.ldd + n, v, (int)min(4ll, a.ldd - n), a.accumulate);
+      }
+    }
+  }
+}
+
+// dst [M][cols] = scale * sum over the slabs [splits][M][ld]; rows to ignore are zero
+__global__ __launch_bounds__(256) void lx_slab_kernel(const float* __restrict__ slab, int splits, int M, int ld,
+                                                      void* __restrict__ dst, int dst_f32, int cols,
+                                                      const float* __restrict__ gloss,
+                                                      const float* __restrict__ inv_count,
+                                                      const long long* __restrict__ target, long long ignore) {
+  const float sc = gloss[0] * inv_count[0];
+  const int c4 = ld >> 2;
+  const long long total = (long long)M * c4, step = (long long)M * ld;
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+    const int r = (int)(i / c4), c = (int)(i - (long long)r * c4) * 4;
+    if (c >= cols) continue;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    if (target[r] != ignore) {
+      const float* s = slab + (long long)r * ld + c;
+      for (int z = 0; z < splits; ++z) {
+        const float4 t = *reinterpret_cast<const float4*>(s + z * step);
+        v[0] += t.x;
+        v[1] += t.y;
+        v[2] += t.z;
+        v[3] += t.w;
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] *= sc;
+    }
+    st4(dst, dst_f32, (long long)r * cols + c, v, min(4, cols - c), false);
+  }
+}
+
+// db [V] = or += scale * column sums of dbpart [tiles][ldp]
+__global__ __launch_bounds__(256) void lx_db_kernel(const float* __restrict__ part, int tiles, int ldp, int V,
+                                                    void* __restrict__ db, int f32, int accumulate,
+                                                    const float* __restrict__ gloss,
+                                                    const float* __restrict__ inv_count) {
+  const int n = blockIdx.x * 256 + threadIdx.x;
+  if (n >= V) return;
+  float s = 0.f;
+  for (int t = 0; t < tiles; ++t) s += part[(long long)t * ldp + n];
+  s *= gloss[0] * inv_count[0];
+  if (f32) {
+    float* d = static_cast<float*>(db) + n;
+    *d = accumulate ? *d + s : s;
+  } else {
+    static_cast<bf16_t*>(db)[n] = f2bf(s);
+  }
+}
+
+// ------------------------------------------------------------------- host
+template <int PL, bool TA, bool TB>
+struct LxTiles {  // 256 only for one plane: three planes of it would not fit LDS twice
+  typedef Gemm<128, 128, 2, 2, PL == 1 ? 64 : 32, 2, PL, TA, TB, false> Mid;
+  typedef Gemm<64, 64, 2, 2, PL == 1 ? 64 : 32, 2, PL, TA, TB, false> Small;
+};
+template <bool TA, bool TB>
+using LxBig = Gemm<256, 256, 2, 4, 64, 2, 1, TA, TB, false>;
+
+inline long long tiles_of(long long m, long long n, int t) { return ((m + t - 1) / t) * ((n + t - 1) / t); }
+
+// Tile of an m x n product (times the splits of its reduction): the largest that still gives the 256
+// compute units a block each, else the smallest.
+inline int pick_tile(long long m, long long n, int splits, int pl) {
+  if (pl == 1 && tiles_of(m, n, 256) * splits >= 192) return 256;
+  if (tiles_of(m, n, 128) * splits >= 192) return 128;
+  return 64;
+}
+
+template <int PL, bool TA, bool TB, typename F>
+int with_tile(int tile, F&& f) {
+  if constexpr (PL == 1)
+    if (tile == 256) return f(LxBig<TA, TB>{});
+  if (tile == 128) return f(typename LxTiles<PL, TA, TB>::Mid{});
+  return f(typename LxTiles<PL, TA, TB>::Small{});
+}
+
+inline int grid_cap(long long n, int cap) {
+  if (n > cap) n = cap;
+  return n < 1 ? 1 : (int)n;
+}
+
+struct LxPlan {
+  int Dp;                   // features, padded to 8
+  bool w_direct;            // the weight is read in place
+  int fwd_tile, fwd_ct;     // forward tile and column tiles
+  int piece, pieces;        // classes of a piece (multiple of 64 unless it is all of V), pieces
+  int bwd_tile, bwd_rt;     // tile and row tiles of the recomputation
+  int dx_tile, dx_splits, dx_ksplit, dw_tile;
+};
+
+inline int up(long long v, int m) { return (int)((v + m - 1) / m * m); }
+
+LxPlan lx_plan(const LxShape& s) {
+  LxPlan p;
+  p.Dp = up(s.D, 8);
+  p.w_direct = s.planes == 1 && !s.w_f32 && s.D % 8 == 0 && s.w_aligned;
+  p.fwd_tile = pick_tile(s.N, s.V, 1, s.planes);
+  p.fwd_ct = (s.V + p.fwd_tile - 1) / p.fwd_tile;
+  const int vp = up(s.V, 64);
+  long long piece = kPieceBytes / (2ll * s.planes * s.N) / 256 * 256;
+  if (piece < 1024) piece = 1024;
+  if (piece > (1 << 20)) piece = 1 << 20;  // a tile's offsets within the piece stay below 2^31 bytes
+  p.piece = piece < vp ? (int)piece : vp;
+  p.pieces = (s.V + p.piece - 1) / p.piece;
+  p.bwd_tile = pick_tile(s.N, p.piece, 1, s.planes);
+  p.bwd_rt = (s.N + p.bwd_tile - 1) / p.bwd_tile;
+  p.dw_tile = pick_tile(p.piece, p.Dp, 1, s.planes);
+  // dx reduces over the classes: split them until the compute units are full, at least 512 a split
+  p.dx_tile = pick_tile(s.N, p.Dp, (int)(p.piece / 512 > 0 ? p.piece / 512 : 1), s.planes);
+  const long long t = tiles_of(s.N, p.Dp, p.dx_tile);
+  long long sp = (384 + t - 1) / t;
+  if (sp > p.piece / 512) sp = p.piece / 512;
+  if (sp < 1) sp = 1;
+  p.dx_ksplit = up((p.piece + sp - 1) / sp, 64);
+  p.dx_splits = (p.piece + p.dx_ksplit - 1) / p.dx_ksplit;
+  return p;
+}
+
+// workspace layout (bytes, 256-aligned)
+struct Carver {
+  char* base;
+  long long off = 0;
+  template <typename T>
+  T* take(long long n) {
+    T* p = reinterpret_cast<T*>(base + off);
+    off += (n * (long long)sizeof(T) + 255) / 256 * 256;
+    return base ? p : nullptr;
+  }
+};
+
+struct LxBuf {
+  bf16_t *x, *w;
+  float *pmax, *psum, *tlogit, *rloss;
+  int *pidx, *hit;
+  bf16_t* prob;
+  float *dbpart, *slab;
+};
+
+LxBuf lx_carve(const LxShape& s, const LxPlan& p, bool bwd, char* base, long long* bytes) {
+  Carver c{base};
+  LxBuf b{};
+  b.x = c.take<bf16_t>((long long)s.planes * s.N * p.Dp);
+  if (!p.w_direct) b.w = c.take<bf16_t>((long long)s.planes * s.V * p.Dp);
+  if (!bwd) {
+    const long long n = (long long)p.fwd_ct * s.N;
+    b.pmax = c.take<float>(n);
+    b.psum = c.take<float>(n);
+    b.pidx = c.take<int>(n);
+    b.tlogit = c.take<float>(s.N);
+    b.rloss = c.take<float>(s.N);
+    b.hit = c.take<int>(s.N);
+  } else {
+    b.prob = c.take<bf16_t>((long long)s.planes * s.N * p.piece);
+    b.dbpart = c.take<float>((long long)p.bwd_rt * p.piece);
+    b.slab = c.take<float>((long long)p.dx_splits * s.N * p.Dp);
+  }
+  *bytes = c.off;
+  return b;
+}
+
+template <int PL>
+GemmOperand<PL> planes_of(const bf16_t* p, long long plane, long long ld, int rows) {
+  GemmOperand<PL> o;
+  for (int q = 0; q < PL; ++q) o.plane[q] = p + q * plane;
+  o.ld = ld;
+  o.rows = rows;
+  return o;
+}
+
+template <int PL>
+void lx_prep(const void* src, bool f32, int rows, int cols, bf16_t* dst, int ld, const long long* target,
+             long long ignore, hipStream_t st) {
+  const long long n = (long long)rows * (ld / 8);
+  hipLaunchKernelGGL(lx_prep_kernel<PL>, dim3(grid_cap((n + 255) / 256, 8192)), dim3(256), 0, st, src, f32 ? 1 : 0,
+                     (long long)cols, rows, cols, dst, (long long)rows * ld, ld, target, ignore);
+}
+
+bool lx_ok(const LxShape& s) {
+  return s.N >= 1 && s.V >= 1 && s.D >= 1 && (s.planes == 1 || s.planes == 3) && s.D <= kGemmMaxLd - 8 &&
+         s.V <= (1 << 30) && s.N <= (1 << 24);
+}
+
+template <int PL>
+int lx_fwd_t(const LxShape& s, const LxIo& io, hipStream_t st) {
+  const LxPlan p = lx_plan(s);
+  long long bytes;
+  const LxBuf b = lx_carve(s, p, false, static_cast<char*>(io.ws), &bytes);
+  lx_prep<PL>(io.x, s.x_f32, s.N, s.D, b.x, p.Dp, io.target, io.ignore, st);
+  if (!p.w_direct) lx_prep<PL>(io.w, s.w_f32, s.V, s.D, b.w, p.Dp, nullptr, 0, st);
+  LxArgs<PL> a{};
+  a.x = planes_of<PL>(b.x, (long long)s.N * p.Dp, p.Dp, s.N);
+  a.w = p.w_direct ? planes_of<PL>(static_cast<const bf16_t*>(io.w), 0, s.D, s.V)
+                   : planes_of<PL>(b.w, (long long)s.V * p.Dp, p.Dp, s.V);
+  a.N = s.N; a.V = s.V; a.D = p.Dp;
+  a.bias = io.bias; a.bias_f32 = s.b_f32;
+  a.target = io.target; a.ignore = io.ignore;
+  a.pmax = b.pmax; a.psum = b.psum; a.pidx = b.pidx; a.tlogit = b.tlogit;
+  const int rc = with_tile<PL, false, false>(p.fwd_tile, [&](auto g) {
+    using G = decltype(g);
+    hipLaunchKernelGGL(lx_fwd_kernel<G>, dim3((unsigned)tiles_of(s.N, s.V, G::BM)), dim3(G::NT), 0, st, a);
+    return 0;
+  });
+  if (rc) return rc;
+  hipLaunchKernelGGL(lx_combine_kernel, dim3((s.N + 15) / 16), dim3(256), 0, st, b.pmax, b.psum, b.pidx, b.tlogit,
+                     io.target, io.ignore, s.N, s.V, p.fwd_ct, io.lse, b.rloss, b.hit);
+  hipLaunchKernelGGL(lx_loss_kernel, dim3(1), dim3(1024), 0, st, b.rloss, b.hit, s.N, io.loss, io.correct,
+                     io.inv_count);
+  return 0;
+}
+
+template <int PL>
+int lx_bwd_t(const LxShape& s, const LxIo& io, hipStream_t st) {
+  const LxPlan p = lx_plan(s);
+  long long bytes;
+  const LxBuf b = lx_carve(s, p, true, static_cast<char*>(io.ws), &bytes);
+  lx_prep<PL>(io.x, s.x_f32, s.N, s.D, b.x, p.Dp, io.target, io.ignore, st);
+  if (!p.w_direct) lx_prep<PL>(io.w, s.w_f32, s.V, s.D, b.w, p.Dp, nullptr, 0, st);
+  const bf16_t* wbase = p.w_direct ? static_cast<const bf16_t*>(io.w) : b.w;
+  const long long wplane = p.w_direct ? 0 : (long long)s.V * p.Dp;
+  for (int k = 0; k < p.pieces; ++k) {
+    const int v0 = k * p.piece, V = s.V - v0 < p.piece ? s.V - v0 : p.piece;
+    LxArgs<PL> a{};
+    a.x = planes_of<PL>(b.x, (long long)s.N * p.Dp, p.Dp, s.N);
+    a.w = planes_of<PL>(wbase + (long long)v0 * p.Dp, wplane, p.Dp, V);
+    a.N = s.N; a.V = V; a.D = p.Dp; a.v0 = v0;
+    const int bsz = s.b_f32 ? 4 : 2;
+    a.bias = io.bias ? static_cast<const char*>(io.bias) + (long long)v0 * bsz : nullptr;
+    a.bias_f32 = s.b_f32;
+    a.target = io.target; a.ignore = io.ignore; a.lse = io.lse;
+    a.ldp = up(V, 64);
+    a.prob = b.prob; a.pplane = (long long)s.N * a.ldp;
+    a.dbpart = io.db ? b.dbpart : nullptr;
+    with_tile<PL, false, false>(p.bwd_tile, [&](auto g) {
+      using G = decltype(g);
+      hipLaunchKernelGGL(lx_prob_kernel<G>, dim3((unsigned)tiles_of(s.N, a.ldp, G::BM)), dim3(G::NT), 0, st, a);
+      return 0;
+    });
+    if (io.db)
+      hipLaunchKernelGGL(lx_db_kernel, dim3((V + 255) / 256), dim3(256), 0, st, b.dbpart, p.bwd_rt, a.ldp, V,
+                         static_cast<void*>(static_cast<char*>(io.db) + (long long)v0 * (s.b_f32 ? 4 : 2)),
+                         s.b_f32 ? 1 : 0, io.accumulate ? 1 : 0, io.gloss, io.inv_count);
+    if (io.dx) {  // slabs [splits][N][Dp] += prob W
+      LxGradArgs<PL> d{};
+      d.A = planes_of<PL>(b.prob, a.pplane, a.ldp, s.N);
+      d.B = planes_of<PL>(wbase + (long long)v0 * p.Dp, wplane, p.Dp, p.Dp);
+      d.M = s.N; d.N = p.Dp; d.K = V; d.ksplit = p.dx_ksplit;
+      d.slab = b.slab; d.slab_add = k > 0;
+      with_tile<PL, false, true>(p.dx_tile, [&](auto g) {
+        using G = decltype(g);
+        hipLaunchKernelGGL(lx_grad_kernel<G>, dim3((unsigned)tiles_of(s.N, p.Dp, G::BM), p.dx_splits), dim3(G::NT), 0,
+                           st, d);
+        return 0;
+      });
+    }
+    if (io.dw) {  // dW[v0 ..] = or += scale prob^T x
+      LxGradArgs<PL> d{};
+      d.A = planes_of<PL>(b.prob, a.pplane, a.ldp, a.ldp);
+      d.B = planes_of<PL>(b.x, (long long)s.N * p.Dp, p.Dp, p.Dp);
+      d.M = V; d.N = p.Dp; d.K = s.N; d.ksplit = up(s.N, 64);
+      d.dst = static_cast<char*>(io.dw) + (long long)v0 * s.D * (io.dw_f32 ? 4 : 2);
+      d.ldd = s.D; d.dst_f32 = io.dw_f32; d.accumulate = io.accumulate;
+      d.gloss = io.gloss; d.inv_count = io.inv_count;
+      with_tile<PL, true, true>(p.dw_tile, [&](auto g) {
+        using G = decltype(g);
+        hipLaunchKernelGGL(lx_grad_kernel<G>, dim3((unsigned)tiles_of(V, p.Dp, G::BM)), dim3(G::NT), 0, st, d);
+        return 0;
+      });
+    }
+  }
+  if (io.dx) {
+    const long long n = (long long)s.N * (p.Dp / 4);
+    hipLaunchKernelGGL(lx_slab_kernel, dim3(grid_cap((n + 255) / 256, 4096)), dim3(256), 0, st, b.slab, p.dx_splits,
+                       s.N, p.Dp, io.dx, s.x_f32 ? 1 : 0, s.D, io.gloss, io.inv_count, io.target, io.ignore);
+  }
+  return 0;
+}
+
+}  // namespace
+
+long long lx_workspace_bytes(const LxShape& s, bool bwd) {
+  if (!lx_ok(s)) return 0;
+  long long bytes;
+  lx_carve(s, lx_plan(s), bwd, nullptr, &bytes);
+  return bytes;
+}
+
+int lx_fwd_launch(const LxShape& s, const LxIo& io, hipStream_t st) {
+  if (!lx_ok(s)) return 1;
+  return s.planes == 1 ? lx_fwd_t<1>(s, io, st) : lx_fwd_t<3>(s, io, st);
+}
+
+int lx_bwd_launch(const LxShape& s, const LxIo& io, hipStream_t st) {
+  if (!lx_ok(s)) return 1;
+  return s.planes == 1 ? lx_bwd_t<1>(s, io, st) : lx_bwd_t<3>(s, io, st);
+}
+
+}  // namespace pmd

@@ -1682,6 +1682,78 @@ def cross_entropy(logits, target):
     return _XentFn.apply(logits, target)
 
 
+class _LinearXentFn(torch.autograd.Function):
+    """(loss, correct) of a linear classifier without its logits; saves the operands and one
+    log-sum-exp per row, and computes the logits again, piece by piece, in the backward."""
+
+    @staticmethod
+    def forward(ctx, x, w, b, target, ignore, bf16):
+        P = prims_for(x)
+        loss, correct, lse, inv = P.linear_xent_fwd(x, w, b, target, ignore, bf16)
+        ctx.save_for_backward(x, w, b, target, lse, inv)
+        ctx.params = (w, b)
+        ctx.cfg = (ignore, bf16)
+        ctx.mark_non_differentiable(correct)
+        ctx.set_materialize_grads(False)
+        return loss.reshape(()), correct
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gloss, _gcorrect):
+        if gloss is None:
+            return (None,) * 6
+        x, w, b, target, lse, inv = ctx.saved_tensors
+        wp, bp = ctx.params
+        ignore, bf16 = ctx.cfg
+        P = prims_for(x)
+        tw = _grad_target(wp)
+        tb = _grad_target(bp) if bp is not None else None
+        arena = tw is not None and (bp is None or tb is not None)
+        dw = db = None
+        if arena:
+            dw, db = tw, tb
+        else:
+            if ctx.needs_input_grad[1]:
+                dw = torch.empty_like(w, memory_format=torch.contiguous_format)
+            if b is not None and ctx.needs_input_grad[2]:
+                db = torch.empty_like(b)
+        g = gloss.reshape(1).to(lse.dtype)
+        dx = P.linear_xent_bwd(g, x, w, b, target, ignore, bf16, lse, inv, ctx.needs_input_grad[0], dw, db, arena)
+        if arena:
+            _ready(wp, *([bp] if bp is not None else []))
+            dw = db = None
+        return dx, dw, db, None, None, None
+
+
+def linear_cross_entropy(x, lin, target, ignore_index=-100, compute_dtype=None):
+    """``(loss, correct)`` of the classifier ``lin`` on features ``x``: the mean softmax cross-entropy of
+    ``x lin.weight^T + lin.bias`` and the top-1 count (int64 [1], on the device) -- what
+    :func:`linear`, :func:`cross_entropy` and :func:`correct_count` give, without keeping the [N, V]
+    logits: for classifiers of many classes.
+
+    ``x`` [..., D] and ``target`` [...] (int64 class indices); rows whose target is ``ignore_index`` count
+    for nothing, whatever they hold, and get a zero gradient; when no row is left the loss is 0.  A
+    target outside the classes makes the loss NaN.  ``lin`` is a module with ``weight`` [V, D] and
+    ``bias`` [V] or None (``torch.nn.Linear``).
+
+    On a GPU operands are bf16 or fp32.  When both are bf16, or with ``compute_dtype=torch.bfloat16``
+    (fp32 operands are then rounded to bf16 first, as :func:`linear` does), products run on bf16 and
+    softmax - onehot is rounded to bf16 for the gradient products; otherwise both keep fp32's 24 bits.
+    Sums are in fp32 always.  Gradients come in their operand's type."""
+    if compute_dtype not in (None, torch.bfloat16):
+        raise ValueError(f"compute_dtype must be None or torch.bfloat16, got {compute_dtype}")
+    w, b = lin.weight, getattr(lin, "bias", None)
+    if x.dim() < 1 or x.shape[-1] != w.shape[1]:
+        raise ValueError(f"x must be [..., {w.shape[1]}], got {tuple(x.shape)}")
+    if target.shape != x.shape[:-1]:
+        raise ValueError(f"target must be {tuple(x.shape[:-1])}, got {tuple(target.shape)}")
+    if target.dtype != torch.int64:
+        raise ValueError(f"target must be int64 class indices, got {target.dtype}")
+    return _LinearXentFn.apply(x.reshape(-1, x.shape[-1]).contiguous(), w.contiguous(), b,
+                               target.reshape(-1).contiguous(), int(ignore_index),
+                               compute_dtype is not None)
+
+
 _SEEDS: dict = {}
 
 

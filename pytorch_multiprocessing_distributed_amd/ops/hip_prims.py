@@ -293,6 +293,18 @@ def xent_bwd(gloss, logits, target, lse):
     return g.to(logits.dtype)
 
 
+def linear_xent_fwd(x, w, b, target, ignore, bf16):
+    """-> (loss [1], correct [1], lse [N], 1 / kept rows [1]); no logits are stored."""
+    return tuple(_C.linear_xent_fwd(x, w.detach(), None if b is None else b.detach(), target, int(ignore),
+                                    bool(bf16)))
+
+
+def linear_xent_bwd(gloss, x, w, b, target, ignore, bf16, lse, inv_count, want_dx, dw, db, accumulate):
+    """-> dx or None; ``dw`` / ``db`` (None: not wanted) are written, or added to (fp32 targets)."""
+    return _C.linear_xent_bwd(gloss, x, w.detach(), None if b is None else b.detach(), target, int(ignore),
+                              bool(bf16), lse, inv_count, bool(want_dx), dw, db, bool(accumulate))
+
+
 def correct_count(logits, target):
     return _C.xent_fwd(logits.float().contiguous(), target)[2]
 

@@ -386,6 +386,47 @@ def xent_bwd(gloss, logits, target, lse):
     return (p * (_f(gloss) / lf.shape[0])).to(logits.dtype)
 
 
+def _lx_operands(x, w, b, bf16):
+    def op(t):
+        return _f(t.detach().to(torch.bfloat16) if bf16 and t.dtype != torch.float64 else t.detach())
+    return op(x), op(w), None if b is None else _f(b.detach())
+
+
+def linear_xent_fwd(x, w, b, target, ignore, bf16):
+    """Mean softmax cross-entropy of ``x w^T + b`` over the rows whose target is not ``ignore``:
+    (loss [1], top-1 count [1], lse [N], 1 / kept rows [1]).  No row kept: loss 0.  A target outside
+    the classes makes its row's loss NaN."""
+    xf, wf, bf = _lx_operands(x, w, b, bf16)
+    keep = target != ignore
+    valid = (target >= 0) & (target < w.shape[0])
+    logits = F.linear(torch.where(keep[:, None], xf, torch.zeros_like(xf)), wf, bf)
+    lse = torch.logsumexp(logits, dim=1)
+    t = torch.where(valid & keep, target, torch.zeros_like(target))
+    nan = torch.full_like(lse, float("nan"))
+    rows = torch.where(valid, lse - logits.gather(1, t[:, None])[:, 0], nan)
+    rows = torch.where(keep, rows, torch.zeros_like(rows))
+    inv = 1.0 / keep.sum().clamp_min(1).to(lse.dtype).reshape(1)
+    correct = torch.zeros(1, dtype=torch.int64, device=x.device)
+    if x.shape[0]:
+        correct = ((logits.argmax(1) == target) & keep).sum().reshape(1)
+    return rows.sum().reshape(1) * inv, correct, torch.where(keep & ~valid, nan, lse), inv
+
+
+def linear_xent_bwd(gloss, x, w, b, target, ignore, bf16, lse, inv_count, want_dx, dw, db, accumulate):
+    """-> dx or None; ``dw`` / ``db`` (None: not wanted) are written, or added to."""
+    xf, wf, bf = _lx_operands(x, w, b, bf16)
+    keep = target != ignore
+    xf = torch.where(keep[:, None], xf, torch.zeros_like(xf))
+    p = torch.exp(F.linear(xf, wf, bf) - lse[:, None])
+    valid = (target >= 0) & (target < w.shape[0]) & keep
+    p[torch.nonzero(valid)[:, 0], target[valid]] -= 1.0
+    p = torch.where(keep[:, None], p, torch.zeros_like(p)) * (_f(gloss) * inv_count)
+    for tgt, g in ((dw, lambda: p.t() @ xf), (db, lambda: p.sum(0))):
+        if tgt is not None:
+            tgt.add_(g().to(tgt.dtype)) if accumulate else tgt.copy_(g())
+    return torch.where(keep[:, None], p @ wf, torch.zeros_like(xf)).to(x.dtype) if want_dx else None
+
+
 def correct_count(logits, target):
     return (logits.argmax(1) == target).sum().to(torch.int64).reshape(1)
 
