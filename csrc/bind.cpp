@@ -955,6 +955,41 @@ Tensor linear_xent_bwd(Tensor gloss, Tensor x, Tensor w, c10::optional<Tensor> b
   return dx;
 }
 
+// ------------------------------------------------------- Newton-Schulz
+// dst[i] = beta dst[i] + alpha[i] (alpha_dev) NS(src[i]); all matrices [m, n] contiguous, one type and device
+void newton_schulz(std::vector<Tensor> src, std::vector<Tensor> dst, int64_t steps, double a, double b, double c,
+                   double eps, std::vector<double> alpha, double beta, c10::optional<Tensor> alpha_dev) {
+  TORCH_CHECK(src.size() == dst.size() && src.size() == alpha.size(), "newton_schulz: one dst and alpha per matrix");
+  if (src.empty()) return;
+  CHECK_DEV(src[0]);
+  const bool f32 = act_esize(src[0], "newton_schulz: a matrix") == 4;
+  const int rc = pmd::ns_check((int)std::max<int64_t>(0, std::min<int64_t>(steps, 1 << 20)), (float)a, (float)b, (float)c);
+  TORCH_CHECK(rc != 1, "newton_schulz: 1 to ", pmd::kNsMaxSteps, " steps, got ", steps);
+  TORCH_CHECK(rc == 0, "newton_schulz: with these coefficients singular values leave the range of 0 to 1024");
+  TORCH_CHECK(eps >= 0 && std::isfinite(eps), "newton_schulz: eps must be finite and not negative");
+  std::vector<pmd::NsMatrix> m;
+  for (size_t i = 0; i < src.size(); ++i) {
+    const Tensor &s = src[i], &d = dst[i];
+    TORCH_CHECK(s.dim() == 2 && s.is_contiguous() && s.device() == src[0].device() &&
+                s.scalar_type() == src[0].scalar_type(),
+                "newton_schulz: matrices must be contiguous [m, n] of one type on one device");
+    TORCH_CHECK(d.sizes() == s.sizes() && d.is_contiguous() && d.device() == s.device() &&
+                d.scalar_type() == s.scalar_type(), "newton_schulz: destination must match its matrix");
+    TORCH_CHECK(s.size(0) <= pmd::kNsMaxSide && s.size(1) <= pmd::kNsMaxSide, "newton_schulz: sides of at most ",
+                pmd::kNsMaxSide);
+    if (s.numel() == 0) continue;
+    m.push_back(pmd::NsMatrix{s.data_ptr(), d.data_ptr(), (int)s.size(0), (int)s.size(1), (float)alpha[i]});
+  }
+  if (m.empty()) return;
+  c10::DeviceGuard g(src[0].device());
+  Tensor ws = torch::empty({pmd::ns_workspace_bytes(m.data(), (int)m.size())}, src[0].options().dtype(torch::kUInt8));
+  const float* ad = opt_f32(alpha_dev, "newton_schulz: alpha_dev");
+  TORCH_CHECK(!ad || alpha_dev->device() == src[0].device(), "newton_schulz: alpha_dev must be on the matrices' device");
+  CHECK_RC(pmd::ns_launch(m.data(), (int)m.size(), f32, (int)steps, (float)a, (float)b, (float)c, (float)eps,
+                          (float)beta, ad, ws.data_ptr(), cur_stream()),
+           "newton_schulz");
+}
+
 // ----------------------------------------------------------------- pools
 std::vector<Tensor> maxpool_fwd(Tensor x) {
   CHECK_DEV(x); CHECK_BF16(x); CHECK_CONT(x);
@@ -1437,6 +1472,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("group_norm_bwd", &group_norm_bwd);
   m.def("linear_xent_fwd", &linear_xent_fwd);
   m.def("linear_xent_bwd", &linear_xent_bwd);
+  m.def("newton_schulz", &newton_schulz);
   m.def("maxpool_fwd", &maxpool_fwd);
   m.def("maxpool_bwd", &maxpool_bwd);
   m.def("stem_pool_fwd", &stem_pool_fwd);

@@ -213,6 +213,22 @@ long long lx_workspace_bytes(const LxShape& s, bool bwd);
 int lx_fwd_launch(const LxShape& s, const LxIo& io, hipStream_t st);
 int lx_bwd_launch(const LxShape& s, const LxIo& io, hipStream_t st);
 
+// Newton-Schulz orthogonalisation, grouped over matrices (kernels/newton_schulz.hip)
+constexpr int kNsGroup = 48;           // matrices per launch (their descriptions travel as kernel arguments)
+constexpr int kNsMaxSteps = 64;
+constexpr int kNsMaxSide = 1 << 20;
+struct NsMatrix {
+  const void* src;                     // [rows][cols]
+  void* dst;                           // [rows][cols], may be src
+  int rows, cols;
+  float alpha;                         // dst = beta dst + alpha X
+};
+// 0, or 1: steps out of range, 2: the coefficients let the singular values grow past fp16's range
+int ns_check(int steps, float a, float b, float c);
+long long ns_workspace_bytes(const NsMatrix* mats, int n);
+int ns_launch(const NsMatrix* mats, int n, bool f32, int steps, float a, float b, float c, float eps, float beta,
+              const float* alpha_dev, void* ws, hipStream_t st);
+
 int zero_launch(void* ptr, long long nbytes, hipStream_t st);  // memset 0 (framework kernel)
 int sgd_launch(float* p, const float* g, float* buf, long long n, float lr, const float* lr_dev,
                float momentum, float wd, float damp, bool nesterov, bool first, hipStream_t st);

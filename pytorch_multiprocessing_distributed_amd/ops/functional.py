@@ -1771,3 +1771,41 @@ def loss_seed(loss):
 def correct_count(logits, target):
     """Device-side top-1 correct count (int64 [1]); no host sync."""
     return prims_for(logits).correct_count(logits, target)
+
+
+# --------------------------------------------------------------------- optim
+NS_COEFFS = (3.4445, -4.7750, 2.0315)    # largest slope at 0 with all singular values ending in 0.7 .. 1.2
+
+
+@torch.no_grad()
+def newton_schulz(update, steps=5, coeffs=NS_COEFFS, eps=1e-7):
+    """The update(s) with their singular values pushed towards 1 by ``steps`` Newton-Schulz steps
+    ``X <- a X + (b S + c S S) X``, ``S = X X^T``, from ``X = U / (|U|_F + eps)``: the direction of the
+    Muon optimizer (``engine.optim.Muon``).
+
+    ``update`` is one tensor or a list of them, each [..., m, n] in bf16 or fp32 (leading dimensions
+    count matrices); the result has the same structure, types and shapes.  All matrices of a type share
+    grouped launches, so hand a model's matrices over in one call.  On a GPU products keep 22 bits
+    (two fp16 planes) whatever the type; the coefficients must keep singular values in [0, 1] below
+    1024.  A zero matrix stays zero.  Not differentiable."""
+    one = torch.is_tensor(update)
+    us = [update] if one else list(update)
+    if int(steps) < 1:
+        raise ValueError(f"newton_schulz needs at least one step, got {steps}")
+    if len(coeffs) != 3:
+        raise ValueError("newton_schulz takes three coefficients")
+    outs, groups = [], {}
+    for u in us:
+        if u.dim() < 2:
+            raise ValueError(f"newton_schulz takes matrices [..., m, n], got {tuple(u.shape)}")
+        u = u.contiguous()
+        out = torch.empty_like(u)
+        outs.append(out)
+        src, dst = groups.setdefault((u.device, u.dtype), ([], []))
+        if u.numel():
+            src.extend(u.flatten(0, -3) if u.dim() > 2 else [u])
+            dst.extend(out.flatten(0, -3) if u.dim() > 2 else [out])
+    for src, dst in groups.values():
+        if src:
+            prims_for(src[0]).newton_schulz_(src, dst, int(steps), coeffs, eps, [1.0] * len(src))
+    return outs[0] if one else outs

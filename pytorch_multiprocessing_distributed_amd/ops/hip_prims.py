@@ -316,6 +316,12 @@ def sgd_nesterov_(params, grads, bufs, lr, momentum, weight_decay, nesterov, fir
             float(dampening), bool(nesterov), bool(first_step), lr_dev)
 
 
+def newton_schulz_(src, dst, steps, coeffs, eps, alpha, beta=0.0, alpha_dev=None):
+    """dst[i] = beta dst[i] + alpha[i] (alpha_dev) NS(src[i]) over [m, n] matrices, grouped launches."""
+    _C.newton_schulz(list(src), list(dst), int(steps), *map(float, coeffs), float(eps), list(alpha), float(beta),
+                     alpha_dev)
+
+
 # ------------------------------------------------------------------- debug
 def _install_sync_debug():
     from ..utils.trace import sync_debug_enabled, wrap_sync_debug

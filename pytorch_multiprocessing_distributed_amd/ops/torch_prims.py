@@ -447,3 +447,23 @@ def sgd_nesterov_(params, grads, bufs, lr, momentum, weight_decay, nesterov, fir
             bufs.mul_(momentum).add_(g, alpha=1.0 - dampening)
         g = g.add(bufs, alpha=momentum) if nesterov else bufs
     params.add_(g, alpha=-lr)
+
+
+def newton_schulz_(src, dst, steps, coeffs, eps, alpha, beta=0.0, alpha_dev=None):
+    """dst[i] = beta dst[i] + alpha[i] (alpha_dev) NS(src[i]) over [m, n] matrices."""
+    a, b, c = coeffs
+    for u, d, al in zip(src, dst, alpha):
+        if u.numel() == 0:
+            continue
+        x = _f(u)
+        tall = x.shape[0] > x.shape[1]
+        if tall:
+            x = x.t()
+        x = x / (x.double().norm().to(x.dtype) + eps)
+        for _ in range(steps):
+            s = x @ x.t()
+            x = a * x + (b * s + c * (s @ s)) @ x
+        x = (x.t() if tall else x) * al
+        if alpha_dev is not None:
+            x = x * alpha_dev
+        d.copy_(x if beta == 0 else _f(d) * beta + x)
