@@ -990,6 +990,28 @@ void newton_schulz(std::vector<Tensor> src, std::vector<Tensor> dst, int64_t ste
            "newton_schulz");
 }
 
+// flat arenas (fp32 [n], n % 4 == 0); kinds uint8 [n / 4]; a rule is (lr, momentum, weight decay, nesterov)
+void muon_prep_(Tensor p, Tensor g, Tensor buf, Tensor upd, Tensor kinds, std::tuple<double, double, double, bool> m,
+                std::tuple<double, double, double, bool> r, c10::optional<Tensor> lr_dev, bool first) {
+  CHECK_DEV(p);
+  for (const Tensor* t : {&p, &g, &buf, &upd})
+    TORCH_CHECK(t->device() == p.device() && t->scalar_type() == torch::kFloat32 && t->is_contiguous() &&
+                t->numel() == p.numel() && reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0,
+                "muon_prep: arenas must be aligned contiguous fp32 tensors of one size on one device");
+  TORCH_CHECK(kinds.device() == p.device() && kinds.scalar_type() == torch::kUInt8 && kinds.is_contiguous() &&
+              kinds.numel() * 4 == p.numel(), "muon_prep: kinds must be uint8 [n / 4]");
+  const float* ld = opt_f32(lr_dev, "muon_prep: lr_dev");
+  TORCH_CHECK(!ld || (lr_dev->numel() == 2 && lr_dev->device() == p.device()), "muon_prep: lr_dev must hold two rates");
+  auto rule = [](const std::tuple<double, double, double, bool>& t) {
+    return pmd::MuonRule{(float)std::get<0>(t), (float)std::get<1>(t), (float)std::get<2>(t), std::get<3>(t) ? 1 : 0};
+  };
+  c10::DeviceGuard guard(p.device());
+  CHECK_RC(pmd::muon_prep_launch(p.data_ptr<float>(), g.data_ptr<float>(), buf.data_ptr<float>(),
+                                 upd.data_ptr<float>(), kinds.data_ptr<uint8_t>(), p.numel(), rule(m), rule(r), ld,
+                                 first, cur_stream()),
+           "muon_prep");
+}
+
 // ----------------------------------------------------------------- pools
 std::vector<Tensor> maxpool_fwd(Tensor x) {
   CHECK_DEV(x); CHECK_BF16(x); CHECK_CONT(x);
@@ -1473,6 +1495,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("linear_xent_fwd", &linear_xent_fwd);
   m.def("linear_xent_bwd", &linear_xent_bwd);
   m.def("newton_schulz", &newton_schulz);
+  m.def("muon_prep_", &muon_prep_);
   m.def("maxpool_fwd", &maxpool_fwd);
   m.def("maxpool_bwd", &maxpool_bwd);
   m.def("stem_pool_fwd", &stem_pool_fwd);

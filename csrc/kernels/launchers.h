@@ -228,6 +228,13 @@ int ns_check(int steps, float a, float b, float c);
 long long ns_workspace_bytes(const NsMatrix* mats, int n);
 int ns_launch(const NsMatrix* mats, int n, bool f32, int steps, float a, float b, float c, float eps, float beta,
               const float* alpha_dev, void* ws, hipStream_t st);
+// momentum of the matrices and the whole step of the rest, over the flat arenas (engine/optim.py Muon)
+struct MuonRule {
+  float lr, momentum, weight_decay;
+  int nesterov;
+};
+int muon_prep_launch(float* p, const float* g, float* buf, float* upd, const uint8_t* kinds, long long n,
+                     const MuonRule& matrices, const MuonRule& rest, const float* lr_dev, bool first, hipStream_t st);
 
 int zero_launch(void* ptr, long long nbytes, hipStream_t st);  // memset 0 (framework kernel)
 int sgd_launch(float* p, const float* g, float* buf, long long n, float lr, const float* lr_dev,

@@ -331,6 +331,44 @@ __global__ __launch_bounds__(G::NT) void ns_update_kernel(NsGroup g, NsIoGroup i
     }
 }
 
+// ------------------------------------------------ the optimizer's first pass
+// One pass over the flat arenas before the orthogonalisation.  kinds [n / 4]: 1 marks matrices
+// (buf = first ? g : mom buf + g, upd = nesterov ? g + mom buf : buf, p *= 1 - lr wd), 0 the rest, which
+// get torch.optim.SGD's whole step here.  Parameters start at multiples of 4 elements.  lr_dev: device
+// learning rates [2] of the two kinds, for captured steps.
+__global__ __launch_bounds__(256) void muon_prep_kernel(float* __restrict__ p, const float* __restrict__ g,
+                                                        float* __restrict__ buf, float* __restrict__ upd,
+                                                        const uint8_t* __restrict__ kinds, long long n4, MuonRule m,
+                                                        MuonRule r, const float* __restrict__ lr_dev, int first) {
+  const float lm = lr_dev ? lr_dev[0] : m.lr, lr = lr_dev ? lr_dev[1] : r.lr;
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n4; i += (long long)gridDim.x * 256) {
+    const bool mat = kinds[i] != 0;
+    const MuonRule k = mat ? m : r;
+    const float4 p4 = reinterpret_cast<const float4*>(p)[i], g4 = reinterpret_cast<const float4*>(g)[i];
+    float pv[4] = {p4.x, p4.y, p4.z, p4.w}, gv[4] = {g4.x, g4.y, g4.z, g4.w}, bv[4] = {0.f, 0.f, 0.f, 0.f};
+    if (!first && k.momentum != 0.f) {
+      const float4 b4 = reinterpret_cast<const float4*>(buf)[i];
+      bv[0] = b4.x;
+      bv[1] = b4.y;
+      bv[2] = b4.z;
+      bv[3] = b4.w;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float d = mat ? gv[e] : gv[e] + k.weight_decay * pv[e];
+      if (k.momentum != 0.f) {
+        bv[e] = first ? d : k.momentum * bv[e] + d;
+        d = k.nesterov ? d + k.momentum * bv[e] : bv[e];
+      }
+      gv[e] = d;
+      pv[e] = mat ? pv[e] * (1.f - lm * k.weight_decay) : pv[e] - lr * d;
+    }
+    if (k.momentum != 0.f) reinterpret_cast<float4*>(buf)[i] = make_float4(bv[0], bv[1], bv[2], bv[3]);
+    if (mat) reinterpret_cast<float4*>(upd)[i] = make_float4(gv[0], gv[1], gv[2], gv[3]);
+    if (!mat || k.weight_decay != 0.f) reinterpret_cast<float4*>(p)[i] = make_float4(pv[0], pv[1], pv[2], pv[3]);
+  }
+}
+
 // ------------------------------------------------------------------- host
 template <bool TB>
 using NsBig = Gemm<256, 256, 2, 4, 32, 2, 2, false, TB, true>;
@@ -460,6 +498,16 @@ long long ns_group_bytes(const NsPlan& p, int n, long long* slab_off, long long*
 }
 
 }  // namespace
+
+int muon_prep_launch(float* p, const float* g, float* buf, float* upd, const uint8_t* kinds, long long n,
+                     const MuonRule& matrices, const MuonRule& rest, const float* lr_dev, bool first, hipStream_t st) {
+  if (n < 0 || n % 4) return 1;
+  if (n == 0) return 0;
+  const long long nb = cdiv(n / 4, 256);
+  hipLaunchKernelGGL(muon_prep_kernel, dim3((int)std::min<long long>(nb, 8192)), dim3(256), 0, st, p, g, buf, upd,
+                     kinds, n / 4, matrices, rest, lr_dev, first ? 1 : 0);
+  return 0;
+}
 
 int ns_check(int steps, float a, float b, float c) {
   NsScales sc[kNsMaxSteps];

@@ -43,6 +43,17 @@ def build_parser():
     p.add_argument("--bucket_mb", default=25.0, type=float)
     p.add_argument("--first_bucket_mb", default=1.0, type=float)
     p.add_argument("--sync_bn", default="on", choices=["on", "off"])
+    p.add_argument("--norm", default="batch", choices=["batch", "group"],
+                   help="group: group norms of 32 groups instead of (Sync)BatchNorm (bf16 or fp32)")
+    p.add_argument("--loss", default="separate", choices=["separate", "fused"],
+                   help="fused: classifier and cross-entropy in one operator that never stores the "
+                        "logits (for many classes)")
+    p.add_argument("--optimizer", default="sgd", choices=["sgd", "muon"],
+                   help="muon: convolution weights along their orthogonalised momentum (--muon_lr, "
+                        "--muon_momentum, --muon_wd), the rest by SGD (--lr, --momentum, --wd)")
+    p.add_argument("--muon_lr", default=0.02, type=float)
+    p.add_argument("--muon_momentum", default=0.95, type=float)
+    p.add_argument("--muon_wd", default=0.0, type=float)
     p.add_argument("--broadcast_buffers", action="store_true",
                    help="re-broadcast BN buffers from rank 0 each forward (reference DDP default)")
     p.add_argument("--lr", default=0.1, type=float)

@@ -25,7 +25,7 @@ from ..parallel.comm import get_comm
 from ..parallel.dp import DataParallel
 from ..utils.checkpoint import load_resume, save_model, save_resume
 from ..utils.logger import DeviceMeter, Logger
-from .optim import FusedSGD
+from .optim import FusedSGD, Muon
 
 
 def _sync(dev):
@@ -91,6 +91,16 @@ def resolve_step_mode(mode, world, on_gpu, image_size, dtype):
     return mode
 
 
+def loss_of(model, inp, target, fused=False):
+    """(loss, top-1 count or None, logits or None) of a batch: the separate operators, or
+    (``--loss fused``) the model's own loss without logits."""
+    if fused:
+        loss, correct = model(inp, target)
+        return loss, correct, None
+    out = model(inp)
+    return OF.cross_entropy(out, target), None, out
+
+
 class GraphedStep:
     """The whole training step (forward, loss, backward, fused SGD) captured ONCE as a HIP graph
     on the current stream and replayed for every later batch of the same shape: the inputs are
@@ -98,7 +108,7 @@ class GraphedStep:
     (``FusedSGD.graph_safe``), and the BN running statistics, statistic slots and gradient
     arena are updated in place by the replay exactly as by an eager step."""
 
-    def __init__(self, model, optimizer, inp, target):
+    def __init__(self, model, optimizer, inp, target, fused=False):
         optimizer.graph_safe()
         self.opt = optimizer
         self.sx = inp.detach().clone()
@@ -107,13 +117,12 @@ class GraphedStep:
         torch.cuda.synchronize()
         self.graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self.graph, stream=torch.cuda.current_stream()):
-            out = model(self.sx)
-            loss = OF.cross_entropy(out, self.sy)
+            loss, self.correct, out = loss_of(model, self.sx, self.sy, fused)
             optimizer.zero_grad()
             loss.backward(OF.loss_seed(loss))
             optimizer.step()
         optimizer.steps -= 1            # the capture recorded the step, it did not run it
-        self.out, self.loss = out.detach(), loss.detach()
+        self.out, self.loss = None if out is None else out.detach(), loss.detach()
 
     def fits(self, inp, target):
         return (tuple(inp.shape), tuple(target.shape)) == self.shape
@@ -147,20 +156,21 @@ def train_epoch(loader, model, optimizer, epoch, logger, args, rank, dev, comm=N
     t_epoch = time.time()
     images = 0
     graphed = getattr(args, "step_mode_resolved", "two_stream") == "graph"
+    fused = getattr(args, "loss", "separate") == "fused"
     for i, (inp, target) in enumerate(loader):
         data_time.update(time.time() - end)
         launch.maybe_inject_fault(rank, step_offset + i)
         g = _graph_of(optimizer) if graphed else None
         if graphed and g is None and step_offset + i >= 2:
             # steps 0-1 ran eagerly: kernel choices tuned, lazy state initialised
-            g = optimizer._pmd_graph = GraphedStep(model, optimizer, inp, target)
+            g = optimizer._pmd_graph = GraphedStep(model, optimizer, inp, target, fused)
         if g is not None and g.fits(inp, target):
             with region("graph"):
                 output, loss = g(inp, target)
+            correct = g.correct
         else:
             with region("fwd"):
-                output = model(inp)
-                loss = OF.cross_entropy(output, target)
+                loss, correct, output = loss_of(model, inp, target, fused)
             optimizer.zero_grad()
             with region("bwd"):
                 loss.backward(OF.loss_seed(loss))
@@ -176,7 +186,8 @@ def train_epoch(loader, model, optimizer, epoch, logger, args, rank, dev, comm=N
             comm.verify_order(model.collective_signature())
         bsz = inp.size(0)
         images += bsz
-        correct = OF.correct_count(output.detach(), target)
+        if correct is None:
+            correct = OF.correct_count(output.detach(), target)
         losses.update(loss.detach(), bsz)
         top1.update(correct.float().squeeze(0) * (100.0 / bsz), bsz)
         if i % args.print_freq == 0 or i == n - 1:
@@ -215,9 +226,8 @@ def validate(loader, model, epoch, logger, args, rank, dev, comm=None, mode="tes
     end = time.time()
     n = len(loader)
     for i, (inp, target) in enumerate(loader):
-        output = model(inp)
-        loss = OF.cross_entropy(output, target)
-        total_correct += OF.correct_count(output, target).double()
+        loss, correct, output = loss_of(model, inp, target, getattr(args, "loss", "separate") == "fused")
+        total_correct += (OF.correct_count(output, target) if correct is None else correct).double()
         seen += target.numel()
         losses.update(loss, inp.size(0))
         batch_time.update(time.time() - end)
@@ -312,9 +322,12 @@ def _run(rank, world_size, args, dev):
             tuning.load(tt)
         elif not tt:
             tuning.load_default()
-    model = build_model(args.model, num_classes=args.num_classes, stem=args.stem).to(dev)
+    norm = getattr(args, "norm", "batch")
+    if norm == "group" and args.dtype == "fp8":
+        raise ValueError("--dtype fp8 needs --norm batch")
+    model = build_model(args.model, num_classes=args.num_classes, stem=args.stem, norm=norm).to(dev)
     comm = get_comm()
-    setup_syncbn(comm, args.sync_bn, getattr(args, "syncbn_comm", "auto"), on_gpu)
+    setup_syncbn(comm, args.sync_bn if norm == "batch" else "off", getattr(args, "syncbn_comm", "auto"), on_gpu)
     args.step_mode_resolved = resolve_step_mode(getattr(args, "step_mode", "auto"), world_size, on_gpu,
                                                 args.image_size, args.dtype)
     OF.set_wgrad_stream(args.step_mode_resolved == "two_stream")
@@ -333,8 +346,12 @@ def _run(rank, world_size, args, dev):
         print("[pmd] gradient buckets (MiB, launch order): "
               + " ".join(f"{m:.2f}" for m in model.bucket_sizes_mb())
               + f" via {model.transport}", flush=True)
-    optimizer = FusedSGD(model, lr=args.lr, momentum=args.momentum, weight_decay=args.wd,
-                         nesterov=True)
+    if getattr(args, "optimizer", "sgd") == "muon":
+        optimizer = Muon(model, lr=args.muon_lr, momentum=args.muon_momentum, weight_decay=args.muon_wd,
+                         rest_lr=args.lr, rest_momentum=args.momentum, rest_weight_decay=args.wd)
+    else:
+        optimizer = FusedSGD(model, lr=args.lr, momentum=args.momentum, weight_decay=args.wd,
+                             nesterov=True)
     scheduler = torch.optim.lr_scheduler.MultiStepLR(optimizer, milestones=args.milestone_list,
                                                      gamma=args.gamma)
     train_logger = Logger(os.path.join(args.save_path, "train.log"))

@@ -84,10 +84,27 @@ def _conv(impl, cin, cout, k, stride, padding):
     return Conv2d(cin, cout, k, stride=stride, padding=padding)
 
 
-def _bn(impl, c):
+GROUPS = 32   # of every norm with norm="group" (the narrowest has 64 channels)
+
+
+def _bn(impl, c, norm="batch"):
+    if norm == "group":
+        return nn.GroupNorm(GROUPS, c)
     if impl == "stock":
         return nn.BatchNorm2d(c)
     return BatchNorm(c)
+
+
+def _group_norm_block(x, stages, final, shortcut):
+    """A residual block with group norms: every conv's output is normalised, activated and, at the
+    end, added to the shortcut in one pass (ops/functional.py group_norm_act)."""
+    h = x
+    for conv, gn in stages:
+        h = OF.group_norm_act(OF.conv(h, conv, want_stats=False)[0], gn)
+    sc = x
+    if shortcut is not None:
+        sc = OF.group_norm_act(OF.conv(x, shortcut[0], want_stats=False)[0], shortcut[1], act="none")
+    return OF.group_norm_act(OF.conv(h, final[0], want_stats=False)[0], final[1], residual=sc)
 
 
 class BasicBlock(nn.Module):
@@ -95,18 +112,19 @@ class BasicBlock(nn.Module):
 
     expansion = 1
 
-    def __init__(self, in_planes, planes, stride=1, impl="fused"):
+    def __init__(self, in_planes, planes, stride=1, impl="fused", norm="batch"):
         super().__init__()
         self.impl = impl
+        self.norm = norm
         self.conv1 = _conv(impl, in_planes, planes, 3, stride, 1)
-        self.bn1 = _bn(impl, planes)
+        self.bn1 = _bn(impl, planes, norm)
         self.conv2 = _conv(impl, planes, planes, 3, 1, 1)
-        self.bn2 = _bn(impl, planes)
+        self.bn2 = _bn(impl, planes, norm)
         self.shortcut = nn.Sequential()
         if stride != 1 or in_planes != self.expansion * planes:
             self.shortcut = nn.Sequential(
                 _conv(impl, in_planes, self.expansion * planes, 1, stride, 0),
-                _bn(impl, self.expansion * planes),
+                _bn(impl, self.expansion * planes, norm),
             )
 
     def forward(self, x):
@@ -116,6 +134,8 @@ class BasicBlock(nn.Module):
             out = out + self.shortcut(x)
             return F.relu(out)
         sc = (self.shortcut[0], self.shortcut[1]) if len(self.shortcut) else None
+        if self.norm == "group":
+            return _group_norm_block(x, [(self.conv1, self.bn1)], (self.conv2, self.bn2), sc)
         return OF.residual_block(x, [(self.conv1, self.bn1)], (self.conv2, self.bn2), sc,
                                  self.bn1.training)
 
@@ -126,20 +146,21 @@ class Bottleneck(nn.Module):
 
     expansion = 4
 
-    def __init__(self, in_planes, planes, stride=1, impl="fused"):
+    def __init__(self, in_planes, planes, stride=1, impl="fused", norm="batch"):
         super().__init__()
         self.impl = impl
+        self.norm = norm
         self.conv1 = _conv(impl, in_planes, planes, 1, 1, 0)
-        self.bn1 = _bn(impl, planes)
+        self.bn1 = _bn(impl, planes, norm)
         self.conv2 = _conv(impl, planes, planes, 3, stride, 1)
-        self.bn2 = _bn(impl, planes)
+        self.bn2 = _bn(impl, planes, norm)
         self.conv3 = _conv(impl, planes, self.expansion * planes, 1, 1, 0)
-        self.bn3 = _bn(impl, self.expansion * planes)
+        self.bn3 = _bn(impl, self.expansion * planes, norm)
         self.shortcut = nn.Sequential()
         if stride != 1 or in_planes != self.expansion * planes:
             self.shortcut = nn.Sequential(
                 _conv(impl, in_planes, self.expansion * planes, 1, stride, 0),
-                _bn(impl, self.expansion * planes),
+                _bn(impl, self.expansion * planes, norm),
             )
 
     def forward(self, x):
@@ -150,6 +171,8 @@ class Bottleneck(nn.Module):
             out = out + self.shortcut(x)
             return F.relu(out)
         sc = (self.shortcut[0], self.shortcut[1]) if len(self.shortcut) else None
+        if self.norm == "group":
+            return _group_norm_block(x, [(self.conv1, self.bn1), (self.conv2, self.bn2)], (self.conv3, self.bn3), sc)
         return OF.residual_block(x, [(self.conv1, self.bn1), (self.conv2, self.bn2)],
                                  (self.conv3, self.bn3), sc, self.bn1.training)
 
@@ -158,13 +181,20 @@ class ResNet(nn.Module):
     """ResNet trunk (reference resnet.py:74-105) with a selectable stem.
 
     Fused-impl input: NHWC ``[N, H, W, C]`` (C may be zero-padded to a
-    multiple of 8 for the MFMA stem); stock-impl input: NCHW."""
+    multiple of 8 for the MFMA stem); stock-impl input: NCHW.
 
-    def __init__(self, block, num_blocks, num_classes=10, stem="cifar", impl="fused"):
+    ``norm="group"``: group norms of 32 groups under the batch norms' names (no running statistics
+    and no exchange between ranks).  Called with a target the fused impl returns ``(loss, correct)``
+    of the classifier (ops/functional.py linear_cross_entropy) instead of the logits."""
+
+    def __init__(self, block, num_blocks, num_classes=10, stem="cifar", impl="fused", norm="batch"):
         super().__init__()
         if stem not in ("cifar", "imagenet"):
             raise ValueError(f"unknown stem {stem!r}")
+        if norm not in ("batch", "group"):
+            raise ValueError(f"unknown norm {norm!r}")
         self.impl = impl
+        self.norm = norm
         self.stem = stem
         self.nchw_input = False   # True: accept reference-style NCHW input and transpose it
         self.in_planes = 64
@@ -172,7 +202,7 @@ class ResNet(nn.Module):
             self.conv1 = _conv(impl, 3, 64, 3, 1, 1)
         else:
             self.conv1 = _conv(impl, 3, 64, 7, 2, 3)
-        self.bn1 = _bn(impl, 64)
+        self.bn1 = _bn(impl, 64, norm)
         self.layer1 = self._make_layer(block, 64, num_blocks[0], stride=1)
         self.layer2 = self._make_layer(block, 128, num_blocks[1], stride=2)
         self.layer3 = self._make_layer(block, 256, num_blocks[2], stride=2)
@@ -183,12 +213,14 @@ class ResNet(nn.Module):
         strides = [stride] + [1] * (num_blocks - 1)
         layers = []
         for s in strides:
-            layers.append(block(self.in_planes, planes, s, impl=self.impl))
+            layers.append(block(self.in_planes, planes, s, impl=self.impl, norm=self.norm))
             self.in_planes = planes * block.expansion
         return nn.Sequential(*layers)
 
-    def forward(self, x):
+    def forward(self, x, target=None):
         if self.impl == "stock":
+            if target is not None:
+                raise ValueError("the stock impl returns logits only")
             out = F.relu(self.bn1(self.conv1(x)))
             if self.stem == "imagenet":
                 out = F.max_pool2d(out, 3, 2, 1)
@@ -198,10 +230,16 @@ class ResNet(nn.Module):
         if self.nchw_input and x.dim() == 4 and x.shape[1] in (3, 8) and x.shape[-1] not in (3, 8):
             x = x.permute(0, 2, 3, 1).contiguous()
         f8 = OF.get_fp8()
+        if f8 is not None and self.norm == "group":
+            raise ValueError("the fp8 convolutions need batch norm: use bf16 with norm='group'")
         if f8 is not None and self.training and torch.is_grad_enabled():
             f8.update()                          # delayed scaling: one device op per step
         with OF.weight_images(self._weight_set(x)):
-            if self.stem == "imagenet" and OF.fused_stem_enabled():
+            if self.norm == "group":
+                out = OF.group_norm_act(OF.conv(x, self.conv1, want_stats=False)[0], self.bn1)
+                if self.stem == "imagenet":
+                    out = OF.max_pool3x3s2(out)
+            elif self.stem == "imagenet" and OF.fused_stem_enabled():
                 # conv1 -> BN -> ReLU -> 3x3/s2 max-pool; the activation is never stored
                 y, s = OF.conv(x, self.conv1, want_stats=self.bn1.training, bn=self.bn1)
                 out = OF.bn_relu_maxpool(y, s, self.bn1)
@@ -211,6 +249,10 @@ class ResNet(nn.Module):
                     out = OF.max_pool3x3s2(out)
             out = self.layer4(self.layer3(self.layer2(self.layer1(out))))
         out = OF.global_avg_pool(out)            # [N, C] fp32
+        if target is not None:
+            # on the GPU operands are rounded to bf16, as OF.linear does
+            return OF.linear_cross_entropy(out, self.linear, target,
+                                           compute_dtype=torch.bfloat16 if out.is_cuda else None)
         return OF.linear(out, self.linear)
 
     def _weight_set(self, x):
@@ -237,8 +279,8 @@ class ResNet(nn.Module):
 
 
 def _factory(block, nb):
-    def make(num_classes=10, stem="cifar", impl="fused"):
-        return ResNet(block, nb, num_classes=num_classes, stem=stem, impl=impl)
+    def make(num_classes=10, stem="cifar", impl="fused", norm="batch"):
+        return ResNet(block, nb, num_classes=num_classes, stem=stem, impl=impl, norm=norm)
     return make
 
 
@@ -256,8 +298,8 @@ MODELS = {
 }
 
 
-def build_model(name, num_classes=10, stem="cifar", impl="fused"):
+def build_model(name, num_classes=10, stem="cifar", impl="fused", norm="batch"):
     key = name.lower()
     if key not in MODELS:
         raise ValueError(f"unknown model {name!r}; choose from {sorted(MODELS)}")
-    return MODELS[key](num_classes=num_classes, stem=stem, impl=impl)
+    return MODELS[key](num_classes=num_classes, stem=stem, impl=impl, norm=norm)

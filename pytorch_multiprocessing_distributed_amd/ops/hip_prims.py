@@ -322,6 +322,12 @@ def newton_schulz_(src, dst, steps, coeffs, eps, alpha, beta=0.0, alpha_dev=None
                      alpha_dev)
 
 
+def muon_prep_(params, grads, bufs, upd, kinds, matrices, rest, lr_dev, first_step):
+    """Momentum of the matrices (into ``upd``) and the whole SGD step of the rest; a rule is (lr,
+    momentum, weight decay, nesterov)."""
+    _C.muon_prep_(params, grads, bufs, upd, kinds, matrices, rest, lr_dev, bool(first_step))
+
+
 # ------------------------------------------------------------------- debug
 def _install_sync_debug():
     from ..utils.trace import sync_debug_enabled, wrap_sync_debug

@@ -467,3 +467,26 @@ def newton_schulz_(src, dst, steps, coeffs, eps, alpha, beta=0.0, alpha_dev=None
         if alpha_dev is not None:
             x = x * alpha_dev
         d.copy_(x if beta == 0 else _f(d) * beta + x)
+
+
+def muon_prep_(params, grads, bufs, upd, kinds, matrices, rest, lr_dev, first_step):
+    """Momentum of the matrices (into ``upd``) and the whole SGD step of the rest, over flat arenas;
+    ``kinds`` (uint8, one per 4 elements) is 1 for matrices; a rule is (lr, momentum, weight decay,
+    nesterov)."""
+    mat = kinds.bool().repeat_interleave(4)
+    for is_mat, (lr, mom, wd, nest) in ((True, matrices), (False, rest)):
+        if lr_dev is not None:
+            lr = float(lr_dev[0 if is_mat else 1].item())
+        m = mat if is_mat else ~mat
+        g = grads if is_mat else grads + wd * params
+        if mom != 0:
+            buf = g if first_step else mom * bufs + g
+            d = g + mom * buf if nest else buf
+            bufs.copy_(torch.where(m, buf, bufs))
+        else:
+            d = g
+        if is_mat:
+            upd.copy_(torch.where(m, d, upd))
+            params.copy_(torch.where(m, params * (1.0 - lr * wd), params))
+        else:
+            params.copy_(torch.where(m, params - lr * d, params))
