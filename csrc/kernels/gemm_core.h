@@ -144,34 +144,131 @@ struct Gemm {
     }
   };
 
-  // fragment of 16 rows x 32 reduction elements: rows r0 + (lane & 15), k = ks * 32 + 8 (lane >> 4) ..
-  template <int ROWS, bool T>
-  static __device__ __forceinline__ s16x8 frag(const char* tile, int r0, int ks, int lane) {
+  // N fragments of 16 rows x 32 reduction elements: rows r0 + 16 i + (lane & 15), k = ks * 32 + 8 (lane >> 4) ..
+  template <int ROWS, bool T, int N>
+  static __device__ __forceinline__ void frags(const char* tile, int r0, int ks, int lane, s16x8 (&f)[N]) {
     if constexpr (!T) {
-      const int row = r0 + (lane & 15), chunk = ks * 4 + (lane >> 4);
-      return *reinterpret_cast<const s16x8*>(tile + row * (BK * 2) + ((chunk ^ swz_rows(row)) << 4));
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int row = r0 + i * 16 + (lane & 15), chunk = ks * 4 + (lane >> 4);
+        f[i] = *reinterpret_cast<const s16x8*>(tile + row * (BK * 2) + ((chunk ^ swz_rows(row)) << 4));
+      }
     } else {
-      const int k = ks * 32 + 8 * (lane >> 4) + ((lane >> 2) & 3), byte = (r0 + 4 * (lane & 3)) * 2;
-      const char* p0 = tile + k * (ROWS * 2) + (((byte >> 5) ^ swz_cols<ROWS>(k)) << 5) + (byte & 31);
-      const char* p1 = tile + (k + 4) * (ROWS * 2) + (((byte >> 5) ^ swz_cols<ROWS>(k + 4)) << 5) + (byte & 31);
-      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p0);
-      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p1);
-      return s16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      const int k = ks * 32 + 8 * (lane >> 4) + ((lane >> 2) & 3);
+      unsigned addr[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int byte = (r0 + i * 16 + 4 * (lane & 3)) * 2;
+        const char* p = tile + k * (ROWS * 2) + (((byte >> 5) ^ swz_cols<ROWS>(k)) << 5) + (byte & 31);
+        addr[i] = (unsigned)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
+      }
+      read_tr<4 * ROWS * 2>(addr, f);  // rows k and k + 4 have the same swizzle
     }
   }
 
+  // Transposed reads, lo halves at the addresses and hi halves OFF bytes further, with their wait: ahead of
+  // the builtin (__builtin_amdgcn_ds_read_tr16_b64_v4i16) the compiler waits for every copy to LDS in
+  // flight, the next step's too, so loads and products took turns.  All of an operand's reads share one wait.
+  template <int OFF>
+  static __device__ __forceinline__ void read_tr(const unsigned (&p)[1], s16x8 (&f)[1]) {
+    s16x4 l0, h0;
+    asm volatile("ds_read_b64_tr_b16 %0, %2\n\tds_read_b64_tr_b16 %1, %2 offset:%3\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(l0), "=&v"(h0) : "v"(p[0]), "n"(OFF));
+    f[0] = join(l0, h0);
+  }
+  template <int OFF>
+  static __device__ __forceinline__ void read_tr(const unsigned (&p)[2], s16x8 (&f)[2]) {
+    s16x4 l0, h0, l1, h1;
+    asm volatile("ds_read_b64_tr_b16 %0, %4\n\tds_read_b64_tr_b16 %1, %4 offset:%6\n\t"
+                 "ds_read_b64_tr_b16 %2, %5\n\tds_read_b64_tr_b16 %3, %5 offset:%6\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(l0), "=&v"(h0), "=&v"(l1), "=&v"(h1) : "v"(p[0]), "v"(p[1]), "n"(OFF));
+    f[0] = join(l0, h0);
+    f[1] = join(l1, h1);
+  }
+  template <int OFF>
+  static __device__ __forceinline__ void read_tr(const unsigned (&p)[4], s16x8 (&f)[4]) {
+    s16x4 l0, h0, l1, h1, l2, h2, l3, h3;
+    asm volatile("ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:%12\n\t"
+                 "ds_read_b64_tr_b16 %2, %9\n\tds_read_b64_tr_b16 %3, %9 offset:%12\n\t"
+                 "ds_read_b64_tr_b16 %4, %10\n\tds_read_b64_tr_b16 %5, %10 offset:%12\n\t"
+                 "ds_read_b64_tr_b16 %6, %11\n\tds_read_b64_tr_b16 %7, %11 offset:%12\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(l0), "=&v"(h0), "=&v"(l1), "=&v"(h1), "=&v"(l2), "=&v"(h2), "=&v"(l3), "=&v"(h3)
+                 : "v"(p[0]), "v"(p[1]), "v"(p[2]), "v"(p[3]), "n"(OFF));
+    f[0] = join(l0, h0);
+    f[1] = join(l1, h1);
+    f[2] = join(l2, h2);
+    f[3] = join(l3, h3);
+  }
+  template <int OFF>
+  static __device__ __forceinline__ void read_tr(const unsigned (&p)[8], s16x8 (&f)[8]) {
+    s16x4 l0, h0, l1, h1, l2, h2, l3, h3, l4, h4, l5, h5, l6, h6, l7, h7;
+    asm volatile("ds_read_b64_tr_b16 %0, %16\n\tds_read_b64_tr_b16 %1, %16 offset:%24\n\t"
+                 "ds_read_b64_tr_b16 %2, %17\n\tds_read_b64_tr_b16 %3, %17 offset:%24\n\t"
+                 "ds_read_b64_tr_b16 %4, %18\n\tds_read_b64_tr_b16 %5, %18 offset:%24\n\t"
+                 "ds_read_b64_tr_b16 %6, %19\n\tds_read_b64_tr_b16 %7, %19 offset:%24\n\t"
+                 "ds_read_b64_tr_b16 %8, %20\n\tds_read_b64_tr_b16 %9, %20 offset:%24\n\t"
+                 "ds_read_b64_tr_b16 %10, %21\n\tds_read_b64_tr_b16 %11, %21 offset:%24\n\t"
+                 "ds_read_b64_tr_b16 %12, %22\n\tds_read_b64_tr_b16 %13, %22 offset:%24\n\t"
+                 "ds_read_b64_tr_b16 %14, %23\n\tds_read_b64_tr_b16 %15, %23 offset:%24\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(l0), "=&v"(h0), "=&v"(l1), "=&v"(h1), "=&v"(l2), "=&v"(h2), "=&v"(l3), "=&v"(h3), "=&v"(l4),
+                   "=&v"(h4), "=&v"(l5), "=&v"(h5), "=&v"(l6), "=&v"(h6), "=&v"(l7), "=&v"(h7)
+                 : "v"(p[0]), "v"(p[1]), "v"(p[2]), "v"(p[3]), "v"(p[4]), "v"(p[5]), "v"(p[6]), "v"(p[7]), "n"(OFF));
+    f[0] = join(l0, h0);
+    f[1] = join(l1, h1);
+    f[2] = join(l2, h2);
+    f[3] = join(l3, h3);
+    f[4] = join(l4, h4);
+    f[5] = join(l5, h5);
+    f[6] = join(l6, h6);
+    f[7] = join(l7, h7);
+  }
+  static __device__ __forceinline__ s16x8 join(const s16x4& l, const s16x4& h) {
+    return s16x8{l[0], l[1], l[2], l[3], h[0], h[1], h[2], h[3]};
+  }
+
+  // `rows` operands: the fragments of one 32-deep slice are read ahead of the MFMAs of the slice before; in
+  // the 256-wide one-plane tile (64 MFMAs a step) the schedule is pinned to a read every second MFMA, which
+  // measured 3-4% over the compiler's own order (reads just ahead of their use): 3.91 against 4.05 ms for
+  // 8,192 x 131,072 x 2,048.
   static __device__ __forceinline__ void step(const char* stage, Acc& acc, int wm, int wn, int lane) {
     const char* At = stage;
     const char* Bt = stage + PL * A_PLANE;
+    if constexpr (PL == 1 && MI * NI == 32 && !TA && !TB) {
+      s16x8 af[2][MI], bf[2][NI];
+#pragma unroll
+      for (int ks = 0; ks <= BK / 32; ++ks) {
+        if (ks < BK / 32) {
+          frags<BN, TB>(Bt, wn * TN, ks, lane, bf[ks & 1]);
+          frags<BM, TA>(At, wm * TM, ks, lane, af[ks & 1]);
+        }
+        if (ks > 0) {
+#pragma unroll
+          for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int j = 0; j < NI; ++j)
+              acc[i][j] = mm16<F16>(bf[(ks - 1) & 1][j], af[(ks - 1) & 1][i], acc[i][j]);
+        }
+      }
+      __builtin_amdgcn_sched_group_barrier(0x100, MI + NI, 0);  // LDS reads of the first slice
+#pragma unroll
+      for (int q = 0; q < MI + NI; ++q) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);  // MFMAs
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
+      return;
+    }
 #pragma unroll
     for (int ks = 0; ks < BK / 32; ++ks) {
       s16x8 af[PL][MI], bf[PL][NI];
 #pragma unroll
-      for (int p = 0; p < PL; ++p) {
-#pragma unroll
-        for (int j = 0; j < NI; ++j) bf[p][j] = frag<BN, TB>(Bt + p * B_PLANE, wn * TN + j * 16, ks, lane);
-#pragma unroll
-        for (int i = 0; i < MI; ++i) af[p][i] = frag<BM, TA>(At + p * A_PLANE, wm * TM + i * 16, ks, lane);
+      for (int p = 0; p < PL; ++p) {  // `rows` operands first: their reads share the others' wait
+        if constexpr (TA) {
+          frags<BN, TB>(Bt + p * B_PLANE, wn * TN, ks, lane, bf[p]);
+          frags<BM, TA>(At + p * A_PLANE, wm * TM, ks, lane, af[p]);
+        } else {
+          frags<BM, TA>(At + p * A_PLANE, wm * TM, ks, lane, af[p]);
+          frags<BN, TB>(Bt + p * B_PLANE, wn * TN, ks, lane, bf[p]);
+        }
       }
       // the smallest products first: they would vanish against a sum that holds the largest
 #pragma unroll
@@ -203,19 +300,19 @@ struct Gemm {
       for (int j = 0; j < NI; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     const Loader ld(A, B, m0, n0, k1, tid);
     constexpr int LPS = PL * (LA + LB);  // loads of a step
+    static_assert(NST >= 2 && NST <= 5 && (NST - 2) * LPS <= 63, "counted waits");
     const int steps = (k1 - k0 + BK - 1) / BK;
 #pragma unroll
     for (int s = 0; s < NST - 1; ++s)
       if (s < steps) ld.load(k0 + s * BK, smem + s * STAGE, wid);
     int buf = 0;
     for (int t = 0; t < steps; ++t) {
-      if constexpr (NST >= 3) {
-        if (t + 1 < steps) wait_loads<(NST - 2) * LPS>();  // steps t+1.. may still be in flight
-        else wait_loads<0>();
-        static_assert(NST <= 3, "the last steps drain one by one");
-      } else {
-        wait_loads<0>();
-      }
+      // step t's copies have landed once at most those of the steps behind it are in flight
+      const int later = min(NST - 2, steps - 1 - t);
+      if (NST >= 5 && later >= 3) wait_loads<3 * LPS>();
+      else if (NST >= 4 && later == 2) wait_loads<2 * LPS>();
+      else if (NST >= 3 && later == 1) wait_loads<LPS>();
+      else wait_loads<0>();
       asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
       if (t + NST - 1 < steps) {
         int nb = buf + NST - 1;

@@ -214,7 +214,7 @@ int lx_fwd_launch(const LxShape& s, const LxIo& io, hipStream_t st);
 int lx_bwd_launch(const LxShape& s, const LxIo& io, hipStream_t st);
 
 // Newton-Schulz orthogonalisation, grouped over matrices (kernels/newton_schulz.hip)
-constexpr int kNsGroup = 48;           // matrices per launch (their descriptions travel as kernel arguments)
+constexpr int kNsGroup = 60;           // matrices per launch (their descriptions travel as kernel arguments)
 constexpr int kNsMaxSteps = 64;
 constexpr int kNsMaxSide = 1 << 20;
 struct NsMatrix {

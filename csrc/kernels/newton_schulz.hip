@@ -23,6 +23,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <vector>
 
 namespace pmd {
 
@@ -30,11 +31,11 @@ namespace {
 
 typedef _Float16 f16_t;
 
+// The matrices of a group, by value in the kernel arguments of the first kernel (which writes the table
+// below) and of the one-block kernel.
 struct NsDim {
   int s, l;          // shorter, longer side
   long long xo, so;  // element offsets in the workspace: X (2 buffers x 2 planes), S and P (2 planes each)
-  int t0;            // first block of this matrix in the phase's grid
-  int splits;        // of the Gram product
 };
 struct NsIo {
   const void* src;
@@ -43,23 +44,63 @@ struct NsIo {
   int tall;          // src is l x s: taken transposed
 };
 struct NsGroup {
-  int count, blocks;
+  int count;
   NsDim d[kNsGroup];
-};
-struct NsIoGroup {
   NsIo io[kNsGroup];
 };
 
-__device__ __forceinline__ int up8(int v) { return (v + 7) & ~7; }
+__host__ __device__ inline int up8(int v) { return (v + 7) & ~7; }
+__host__ __device__ inline long long cdiv(long long a, long long b) { return (a + b - 1) / b; }
+__host__ __device__ inline int tri(int t) { return t * (t + 1) / 2; }
 
-__device__ __forceinline__ int find_matrix(const NsGroup& g, int block) {
-  int lo = 0, hi = g.count - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (g.d[mid].t0 <= block) lo = mid;
-    else hi = mid - 1;
+// How the phases of a group are cut into blocks.
+enum NsPhase { kNorm, kStart, kGram, kJoin, kPoly, kUpdate, kPhases };
+constexpr int kNormBlocks = 256;  // partial sums of a matrix's norm, at most
+struct NsCut {
+  int kc;                                   // reduction of a Gram block
+  int gram_small, poly_small, upd_small;    // 64-wide tiles for all
+  int upd_big;                              // 256-wide tiles for all
+};
+struct NsBlocks {
+  int tile, splits, blocks;  // splits: blocks that share a sum (of a Gram tile, of the norm)
+};
+__host__ __device__ inline NsBlocks ns_blocks(int phase, int s, int l, const NsCut& c) {
+  const int t = s <= 64 ? 64 : 128, lp = up8(l);
+  NsBlocks b{t, 1, 0};
+  if (phase == kNorm) {
+    const long long n = cdiv((long long)s * l, 16384);
+    b.splits = b.blocks = n < kNormBlocks ? (int)n : kNormBlocks;
+  } else if (phase == kStart) {
+    b.blocks = (int)(cdiv(s, 64) * cdiv(lp, 64));
+  } else if (phase == kGram || phase == kJoin) {
+    b.tile = c.gram_small ? 64 : t;
+    b.splits = (int)cdiv(l, c.kc);
+    const int tiles = tri((int)cdiv(s, b.tile));
+    b.blocks = phase == kGram ? tiles * b.splits : b.splits > 1 ? tiles * (b.tile * b.tile / 1024) : 0;
+  } else if (phase == kPoly) {
+    b.tile = c.poly_small ? 64 : t;
+    b.blocks = tri((int)cdiv(s, b.tile));
+  } else {
+    b.tile = c.upd_big ? 256 : c.upd_small ? 64 : t;
+    b.blocks = (int)(cdiv(s, b.tile) * cdiv(lp, b.tile));
   }
-  return lo;
+  return b;
+}
+
+// The same in device memory, for the launches that look up their matrix by block: kernel arguments lie
+// in host memory, where a search costs a microsecond a step (a call's 17 launches over one 512 x 4,608
+// matrix took 282 us with the search in the arguments and take 190 us with it here).
+struct NsTable {
+  int t0[kPhases][64];  // first block of each matrix (past the last matrix: never reached)
+  NsBlocks b[kPhases][kNsGroup];
+  NsDim d[kNsGroup];
+  NsIo io[kNsGroup];
+};
+
+// the matrix of a block: one load and a ballot
+__device__ __forceinline__ int find_matrix(const NsTable* t, int phase, int block) {
+  const unsigned long long m = __ballot(t->t0[phase][threadIdx.x & 63] <= block);
+  return 63 - __clzll(m);
 }
 
 __device__ __forceinline__ float ns_ld(const void* p, long long i, bool f32) {
@@ -76,49 +117,97 @@ __device__ __forceinline__ float join2(unsigned short hi, unsigned short lo) {
 }
 
 // ------------------------------------------------------------- norm, start
-constexpr int kNormBlocks = 64;  // partial sums per matrix
-
 // part [matrix][kNormBlocks] = sums of squares, in fp64 (entries of 1e-30 or 1e30 neither vanish nor
-// overflow)
-__global__ __launch_bounds__(256) void ns_norm_kernel(NsGroup g, NsIoGroup io, int f32, double* __restrict__ part) {
+// overflow); a block takes at least 16,384 elements.  Block 0 also writes the table.
+__global__ __launch_bounds__(256) void ns_norm_kernel(NsGroup g, NsCut cut, int f32, double* __restrict__ part,
+                                                      NsTable* __restrict__ table) {
   __shared__ double red[4];
-  const int k = blockIdx.x / kNormBlocks, b = blockIdx.x % kNormBlocks;
+  __shared__ int first[kNsGroup + 1];
+  if (threadIdx.x == 0) {
+    int t = 0;
+    for (int i = 0; i < g.count; ++i) {
+      first[i] = t;
+      t += ns_blocks(kNorm, g.d[i].s, g.d[i].l, cut).blocks;
+    }
+    first[g.count] = t;
+  }
+  __syncthreads();
+  int k = 0;
+  while (first[k + 1] <= (int)blockIdx.x) ++k;
+  const int b = blockIdx.x - first[k], nb = first[k + 1] - first[k];
+  if (blockIdx.x == 0) {
+    if (threadIdx.x < kPhases) {
+      const int ph = threadIdx.x;
+      int t = 0;
+      for (int i = 0; i < 64; ++i) {
+        table->t0[ph][i] = i < g.count ? t : 0x7fffffff;
+        if (i < g.count) t += (table->b[ph][i] = ns_blocks(ph, g.d[i].s, g.d[i].l, cut)).blocks;
+      }
+    } else if (threadIdx.x >= 64 && threadIdx.x < 64 + g.count) {
+      table->d[threadIdx.x - 64] = g.d[threadIdx.x - 64];
+      table->io[threadIdx.x - 64] = g.io[threadIdx.x - 64];
+    }
+  }
   const long long n = (long long)g.d[k].s * g.d[k].l;
+  const void* src = g.io[k].src;
   double s = 0.0;
-  for (long long i = b * 256ll + threadIdx.x; i < n; i += kNormBlocks * 256ll) {
-    const double v = ns_ld(io.io[k].src, i, f32);
+  const long long n4 = reinterpret_cast<uintptr_t>(src) % 16 == 0 ? n >> 2 : 0;  // whole vectors
+  for (long long i = b * 256ll + threadIdx.x; i < n4; i += nb * 256ll) {
+    float v[4];
+    if (f32) {
+      const float4 t = static_cast<const float4*>(src)[i];
+      v[0] = t.x;
+      v[1] = t.y;
+      v[2] = t.z;
+      v[3] = t.w;
+    } else {
+      const uint2 t = static_cast<const uint2*>(src)[i];
+      v[0] = bf2f(t.x & 0xffff);
+      v[1] = bf2f(t.x >> 16);
+      v[2] = bf2f(t.y & 0xffff);
+      v[3] = bf2f(t.y >> 16);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s += (double)v[e] * v[e];
+  }
+  for (long long i = n4 * 4 + b * 256ll + threadIdx.x; i < n; i += nb * 256ll) {
+    const double v = ns_ld(src, i, f32);
     s += v * v;
   }
   for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
   __syncthreads();
-  if (threadIdx.x == 0) part[blockIdx.x] = ((red[0] + red[1]) + red[2]) + red[3];
+  if (threadIdx.x == 0) part[k * kNormBlocks + b] = ((red[0] + red[1]) + red[2]) + red[3];
 }
 
 // X_0 planes [s][up8(l)] of one 64 x 64 tile, through LDS when the matrix is taken transposed
-__global__ __launch_bounds__(256) void ns_start_kernel(NsGroup g, NsIoGroup io, int f32, const double* __restrict__ part,
-                                                       unsigned short* __restrict__ ws, float eps, float scale) {
+__global__ __launch_bounds__(256) void ns_start_kernel(const NsTable* __restrict__ tab, int f32,
+                                                       const double* __restrict__ part, unsigned short* __restrict__ ws,
+                                                       float eps, float scale) {
   __shared__ float tile[64][65];
   __shared__ float inv_s;
-  const int k = find_matrix(g, blockIdx.x), t = blockIdx.x - g.d[k].t0;
-  const int s = g.d[k].s, l = g.d[k].l, lp = up8(l);
+  const int k = find_matrix(tab, kStart, blockIdx.x), t = blockIdx.x - tab->t0[kStart][k];
+  const NsDim d = tab->d[k];
+  const NsIo io = tab->io[k];
+  const int s = d.s, l = d.l, lp = up8(l), sums = tab->b[kNorm][k].splits;
   const int tl = (lp + 63) / 64, r0 = (t / tl) * 64, c0 = (t % tl) * 64;
   if (threadIdx.x < 64) {
-    double v = part[k * kNormBlocks + threadIdx.x];
+    double v = 0.0;
+    for (int i = threadIdx.x; i < sums; i += 64) v += part[k * kNormBlocks + i];
     for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
     if (threadIdx.x == 0) inv_s = (float)(1.0 / (sqrt(v) + (double)eps)) * scale;
   }
-  const bool tall = io.io[k].tall;
+  const bool tall = io.tall;
   const int a = threadIdx.x & 63, b = threadIdx.x >> 6;
   for (int i = b; i < 64; i += 4) {  // a: along the source's rows
     const int r = tall ? r0 + a : r0 + i, c = tall ? c0 + i : c0 + a;
-    const float v = r < s && c < l ? ns_ld(io.io[k].src, tall ? (long long)c * s + r : (long long)r * l + c, f32) : 0.f;
+    const float v = r < s && c < l ? ns_ld(io.src, tall ? (long long)c * s + r : (long long)r * l + c, f32) : 0.f;
     if (tall) tile[a][i] = v;
     else tile[i][a] = v;
   }
   __syncthreads();
   const float inv = inv_s;
-  unsigned short* x = ws + g.d[k].xo;
+  unsigned short* x = ws + d.xo;
   const long long plane = (long long)s * lp;
   for (int i = b; i < 64; i += 4) {
     const int r = r0 + i, c = c0 + a;
@@ -143,42 +232,93 @@ __device__ __forceinline__ GemmOperand<2> ns_operand(const unsigned short* p, lo
 // tile t of the lower triangle, row by row
 __device__ __forceinline__ void tri_of(int t, int& im, int& in) {
   int r = (int)((sqrtf(8.f * t + 1.f) - 1.f) * 0.5f);
-  while ((long long)(r + 1) * (r + 2) / 2 <= t) ++r;
-  while ((long long)r * (r + 1) / 2 > t) --r;
+  while ((r + 1) * (r + 2) / 2 <= t) ++r;
+  while (r * (r + 1) / 2 > t) --r;
   im = r;
   in = t - r * (r + 1) / 2;
 }
 
-// four neighbours n.. of row m of a symmetric matrix [s][up8(s)] (2 planes), and their mirror images
-__device__ __forceinline__ void put_sym(unsigned short* p, int s, int m, int n, const float (&v)[4], bool mirror) {
-  const int ld = up8(s);
-  const long long plane = (long long)s * ld;
+__device__ __forceinline__ void put_planes(unsigned short* p, long long plane, long long o, const float (&v)[4]) {
   unsigned short h[4], l[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) split2(v[e], h[e], l[e]);
-  if (m < s && n < ld) {
-    const long long o = (long long)m * ld + n;
-    *reinterpret_cast<uint2*>(p + o) = make_uint2(h[0] | ((uint32_t)h[1] << 16), h[2] | ((uint32_t)h[3] << 16));
-    *reinterpret_cast<uint2*>(p + plane + o) = make_uint2(l[0] | ((uint32_t)l[1] << 16), l[2] | ((uint32_t)l[3] << 16));
-  }
-  if (mirror && m < ld)
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (n + e < s) {
-        p[(long long)(n + e) * ld + m] = h[e];
-        p[plane + (long long)(n + e) * ld + m] = l[e];
-      }
+  *reinterpret_cast<uint2*>(p + o) = make_uint2(h[0] | ((uint32_t)h[1] << 16), h[2] | ((uint32_t)h[3] << 16));
+  *reinterpret_cast<uint2*>(p + plane + o) = make_uint2(l[0] | ((uint32_t)l[1] << 16), l[2] | ((uint32_t)l[3] << 16));
 }
 
-// S = X X^T: planes scaled by out_scale / (X's scale)^2 in one go, or slabs [block][BM][BN] (raw sums)
+// four neighbours n.. of row m of a symmetric matrix [s][up8(s)] (2 planes), and their mirror images.
+// Four neighbouring lanes hold four neighbouring rows m; they transpose their 4 x 4 values among
+// themselves, so that the mirror image is stored 8 bytes wide too (all 64 lanes call this, with m and n
+// multiples of 4 apart from the lane's own m & 3).
+__device__ __forceinline__ void put_sym(unsigned short* p, int s, int m, int n, const float (&v)[4], bool mirror) {
+  const int ld = up8(s);
+  const long long plane = (long long)s * ld;
+  if (m < s && n < ld) put_planes(p, plane, (long long)m * ld + n, v);
+  if (!mirror) return;
+  float t[4] = {v[0], v[1], v[2], v[3]};
+  const int q = threadIdx.x & 3;
+#pragma unroll
+  for (int o = 1; o <= 2; o <<= 1) {
+    const bool up = q & o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (!(e & o)) {
+        const float r = __shfl_xor(up ? t[e] : t[e | o], o, 64);
+        if (up) t[e] = r;
+        else t[e | o] = r;
+      }
+  }
+  const int row = n + q, col = m & ~3;  // now t[e] belongs to (m & ~3) + e, n + q
+  if (row < s && col < ld) put_planes(p, plane, (long long)row * ld + col, t);
+}
+
+__device__ __forceinline__ void join4(const uint2& h, const uint2& l, float (&v)[4]) {
+  v[0] = join2(h.x & 0xffff, l.x & 0xffff);
+  v[1] = join2(h.x >> 16, l.x >> 16);
+  v[2] = join2(h.y & 0xffff, l.y & 0xffff);
+  v[3] = join2(h.y >> 16, l.y >> 16);
+}
+
+// An epilogue's rows of 16, in runs short enough that the run's operands (4 registers a tile) fit beside
+// the accumulators: all of a run's loads are issued before the first is used.
+template <class G, typename F>
+__device__ __forceinline__ void for_rows(F&& f) {
+  constexpr int R = G::MI * G::NI > 16 ? 16 / G::NI : G::MI;
+  static_assert(G::MI % R == 0, "whole runs");
+  f(std::integral_constant<int, 0>{}, std::integral_constant<int, R>{});
+  if constexpr (G::MI > R) f(std::integral_constant<int, R>{}, std::integral_constant<int, R>{});
+  static_assert(G::MI <= 2 * R, "two runs");
+}
+
+// the tiles (m + 16 i, n + 16 j) of a matrix in two planes (zero outside [rows][cols])
+template <class G, int R>
+__device__ __forceinline__ void load_planes(const unsigned short* p, long long plane, int ld, int rows, int cols, int m,
+                                            int n, uint2 (&h)[R][G::NI], uint2 (&l)[R][G::NI]) {
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+#pragma unroll
+    for (int j = 0; j < G::NI; ++j) {
+      const bool ok = m + i * 16 < rows && n + j * 16 < cols;
+      const long long o = ok ? (long long)(m + i * 16) * ld + n + j * 16 : 0;
+      const uint2 a = *reinterpret_cast<const uint2*>(p + o), b = *reinterpret_cast<const uint2*>(p + plane + o);
+      h[i][j] = ok ? a : make_uint2(0, 0);
+      l[i][j] = ok ? b : make_uint2(0, 0);
+    }
+}
+
+// The kernels below take their tile per matrix: the grid of a group mixes 128- and 64-wide tiles (G1,
+// G2: 256 threads each), a group of large matrices runs on 256-wide ones alone (G1 = G2).
+template <class G1, class G2>
+constexpr int ns_lds() {
+  return G1::LDS > G2::LDS ? G1::LDS : G2::LDS;
+}
+
+// S = X X^T: planes scaled by out_scale / (X's scale)^2 in one go, or (split sums) slabs
+// [block][BM][BN] of raw sums
 template <class G>
-__global__ __launch_bounds__(G::NT) void ns_gram_kernel(NsGroup g, unsigned short* __restrict__ ws, int xbuf, int kc,
-                                                        float mul, float* __restrict__ slab) {
-  __shared__ __attribute__((aligned(16))) char smem[G::LDS];
-  const int L = xcd_remap(blockIdx.x, gridDim.x);
-  const int k = find_matrix(g, L);
-  const NsDim d = g.d[k];
-  const int r = L - d.t0, t = r / d.splits, z = r - t * d.splits;
+__device__ __forceinline__ void ns_gram_tile(const NsDim& d, int splits, int L, int r, unsigned short* ws, int xbuf,
+                                             int kc, float mul, float* slab, int slab_stride, char* smem) {
+  const int t = r / splits, z = r - t * splits;
   int im, in;
   tri_of(t, im, in);
   const int lp = up8(d.l);
@@ -192,8 +332,8 @@ __global__ __launch_bounds__(G::NT) void ns_gram_kernel(NsGroup g, unsigned shor
 #pragma unroll
     for (int j = 0; j < G::NI; ++j) {
       const int ml = wm * G::TM + i * 16 + (lane & 15), nl = wn * G::TN + j * 16 + (lane >> 4) * 4;
-      if (slab) {
-        *reinterpret_cast<float4*>(slab + ((long long)L * G::BM + ml) * G::BN + nl) =
+      if (splits > 1) {
+        *reinterpret_cast<float4*>(slab + (long long)L * slab_stride + ml * G::BN + nl) =
             make_float4(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]);
       } else {
         const float v[4] = {acc[i][j][0] * mul, acc[i][j][1] * mul, acc[i][j][2] * mul, acc[i][j][3] * mul};
@@ -201,46 +341,51 @@ __global__ __launch_bounds__(G::NT) void ns_gram_kernel(NsGroup g, unsigned shor
       }
     }
 }
+template <class G1, class G2>
+__global__ __launch_bounds__(G1::NT) void ns_gram_kernel(const NsTable* __restrict__ tab,
+                                                         unsigned short* __restrict__ ws, int xbuf, int kc, float mul,
+                                                         float* __restrict__ slab, int slab_stride) {
+  __shared__ __attribute__((aligned(16))) char smem[ns_lds<G1, G2>()];
+  const int L = xcd_remap(blockIdx.x, gridDim.x);
+  const int k = find_matrix(tab, kGram, L), r = L - tab->t0[kGram][k];
+  const NsDim d = tab->d[k];
+  const NsBlocks b = tab->b[kGram][k];
+  if (b.tile == G1::BM) ns_gram_tile<G1>(d, b.splits, L, r, ws, xbuf, kc, mul, slab, slab_stride, smem);
+  else ns_gram_tile<G2>(d, b.splits, L, r, ws, xbuf, kc, mul, slab, slab_stride, smem);
+}
 
-// joins the slabs of the Gram product's tiles in order; 4 blocks a tile
-template <int BT>
-__global__ __launch_bounds__(256) void ns_join_kernel(NsGroup g, unsigned short* __restrict__ ws,
-                                                      const float* __restrict__ slab, float mul) {
-  // g.t0 counts the Gram product's blocks (tile x split); this grid has 4 blocks for every one of
-  // them, and those of a split z > 0 have nothing to do
-  const int b = blockIdx.x >> 2, part = blockIdx.x & 3;
-  const int k = find_matrix(g, b);
-  const NsDim d = g.d[k];
-  const int r = b - d.t0, t = r / d.splits;
-  if (r - t * d.splits != 0) return;
+// joins the slabs of the Gram tiles in order, 1,024 values a block
+__global__ __launch_bounds__(256) void ns_join_kernel(const NsTable* __restrict__ tab, unsigned short* __restrict__ ws,
+                                                      const float* __restrict__ slab, int slab_stride, float mul) {
+  const int k = find_matrix(tab, kJoin, blockIdx.x), b = blockIdx.x - tab->t0[kJoin][k];
+  const NsDim d = tab->d[k];
+  const int BT = tab->b[kJoin][k].tile, splits = tab->b[kJoin][k].splits;
+  const int per = BT * BT / 1024, t = b / per, part = b - t * per;
   int im, in;
   tri_of(t, im, in);
-  const float* s0 = slab + (long long)b * BT * BT;
-  for (int e = threadIdx.x; e < BT * BT / 16; e += 256) {
-    const int i = (part * (BT * BT / 16) + e) * 4;
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int z = 0; z < d.splits; ++z) {
-      const float4 q = *reinterpret_cast<const float4*>(s0 + (long long)z * BT * BT + i);
-      v[0] += q.x;
-      v[1] += q.y;
-      v[2] += q.z;
-      v[3] += q.w;
-    }
-#pragma unroll
-    for (int c = 0; c < 4; ++c) v[c] *= mul;
-    put_sym(ws + d.so, d.s, im * BT + i / BT, in * BT + i % BT, v, im != in);
+  const float* s0 = slab + (tab->t0[kGram][k] + (long long)t * splits) * slab_stride;
+  const int u = part * 256 + threadIdx.x, q = u >> 2;  // four neighbouring lanes: four rows (put_sym)
+  const int m = q / (BT / 4) * 4 + (u & 3), n = q % (BT / 4) * 4;
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int z = 0; z < splits; ++z) {
+    const float4 w = *reinterpret_cast<const float4*>(s0 + (long long)z * slab_stride + m * BT + n);
+    v[0] += w.x;
+    v[1] += w.y;
+    v[2] += w.z;
+    v[3] += w.w;
   }
+#pragma unroll
+  for (int c = 0; c < 4; ++c) v[c] *= mul;
+  put_sym(ws + d.so, d.s, im * BT + m, in * BT + n, v, im != in);
 }
 
 // P = b S + c S S (S's scale ss, P's scale sp)
 template <class G>
-__global__ __launch_bounds__(G::NT) void ns_poly_kernel(NsGroup g, unsigned short* __restrict__ ws, float b, float c,
-                                                        float inv_ss, float sp) {
-  __shared__ __attribute__((aligned(16))) char smem[G::LDS];
-  const int L = xcd_remap(blockIdx.x, gridDim.x);
-  const NsDim d = g.d[find_matrix(g, L)];
+__device__ __forceinline__ void ns_poly_tile(const NsDim& d, int t, unsigned short* ws, float b, float c, float inv_ss,
+                                             float sp, char* smem) {
   int im, in;
-  tri_of(L - d.t0, im, in);
+  tri_of(t, im, in);
   const int ld = up8(d.s);
   const long long plane = (long long)d.s * ld;
   const unsigned short* S = ws + d.so;
@@ -249,35 +394,62 @@ __global__ __launch_bounds__(G::NT) void ns_poly_kernel(NsGroup g, unsigned shor
   G::run(x, x, im * G::BM, in * G::BN, 0, d.s, smem, acc);
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, wm = wid / G::WN, wn = wid % G::WN;
   const float kc = c * inv_ss * inv_ss * sp, kb = b * inv_ss * sp;
+  const int mb = im * G::BM + wm * G::TM + (lane & 15), nb = in * G::BN + wn * G::TN + (lane >> 4) * 4;
+  for_rows<G>([&](auto i0, auto rows) {
+    uint2 h[rows][G::NI], l[rows][G::NI];
+    load_planes<G, rows>(S, plane, ld, d.s, ld, mb + i0 * 16, nb, h, l);
 #pragma unroll
-  for (int i = 0; i < G::MI; ++i)
+    for (int i = 0; i < rows; ++i)
 #pragma unroll
-    for (int j = 0; j < G::NI; ++j) {
-      const int m = im * G::BM + wm * G::TM + i * 16 + (lane & 15);
-      const int n = in * G::BN + wn * G::TN + j * 16 + (lane >> 4) * 4;
-      float v[4] = {0.f, 0.f, 0.f, 0.f};
-      if (m < d.s && n < ld) {
-        const long long o = (long long)m * ld + n;
-        const uint2 h = *reinterpret_cast<const uint2*>(S + o), l = *reinterpret_cast<const uint2*>(S + plane + o);
-        const float sv[4] = {join2(h.x & 0xffff, l.x & 0xffff), join2(h.x >> 16, l.x >> 16),
-                             join2(h.y & 0xffff, l.y & 0xffff), join2(h.y >> 16, l.y >> 16)};
+      for (int j = 0; j < G::NI; ++j) {
+        float sv[4], v[4];
+        join4(h[i][j], l[i][j], sv);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = fmaf(kc, acc[i][j][e], kb * sv[e]);
+        for (int e = 0; e < 4; ++e) v[e] = fmaf(kc, acc[i0 + i][j][e], kb * sv[e]);
+        put_sym(ws + d.so + 2 * plane, d.s, mb + (i0 + i) * 16, nb + j * 16, v, im != in);
       }
-      put_sym(ws + d.so + 2 * plane, d.s, m, n, v, im != in);
-    }
+  });
 }
+template <class G1, class G2>
+__global__ __launch_bounds__(G1::NT) void ns_poly_kernel(const NsTable* __restrict__ tab,
+                                                         unsigned short* __restrict__ ws, float b, float c, float inv_ss,
+                                                         float sp) {
+  __shared__ __attribute__((aligned(16))) char smem[ns_lds<G1, G2>()];
+  const int L = xcd_remap(blockIdx.x, gridDim.x);
+  const int k = find_matrix(tab, kPoly, L), t = L - tab->t0[kPoly][k];
+  const NsDim d = tab->d[k];
+  if (tab->b[kPoly][k].tile == G1::BM) ns_poly_tile<G1>(d, t, ws, b, c, inv_ss, sp, smem);
+  else ns_poly_tile<G2>(d, t, ws, b, c, inv_ss, sp, smem);
+}
+
+// four values (m, n..) of out = beta out + alpha X
+__device__ __forceinline__ void ns_out(const NsIo& io, int f32, int s, int l, int m, int n, const float (&v)[4],
+                                       float alpha, float beta) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (n + e >= l) continue;
+    const long long q = io.tall ? (long long)(n + e) * s + m : (long long)m * l + n + e;
+    if (f32) {
+      float* dst = static_cast<float*>(io.dst) + q;
+      *dst = beta != 0.f ? fmaf(alpha, v[e], beta * *dst) : alpha * v[e];
+    } else {
+      bf16_t* dst = static_cast<bf16_t*>(io.dst) + q;
+      *dst = f2bf(beta != 0.f ? fmaf(alpha, v[e], beta * bf2f(*dst)) : alpha * v[e]);
+    }
+  }
+}
+
+struct NsStep {  // of the update: a, 1 / scales of X and P, scale of the next X; the last step's output
+  float a, inv_sx, inv_sp, so, beta;
+  int f32;
+  const float* alpha_dev;
+};
 
 // X' = a X + P X into the other buffer, or (LAST) out = beta out + alpha X'
 template <class G, bool LAST>
-__global__ __launch_bounds__(G::NT) void ns_update_kernel(NsGroup g, NsIoGroup io, unsigned short* __restrict__ ws,
-                                                          int xbuf, float a, float inv_sx, float inv_sp, float so,
-                                                          int f32, float beta, const float* __restrict__ alpha_dev) {
-  __shared__ __attribute__((aligned(16))) char smem[G::LDS];
-  const int L = xcd_remap(blockIdx.x, gridDim.x);
-  const int k = find_matrix(g, L);
-  const NsDim d = g.d[k];
-  const int t = L - d.t0, lp = up8(d.l), ld = up8(d.s);
+__device__ __forceinline__ void ns_update_tile(const NsDim& d, int t, const NsIo& io, unsigned short* ws, int xbuf,
+                                               const NsStep& st, char* smem) {
+  const int lp = up8(d.l), ld = up8(d.s);
   const int tm = (d.s + G::BM - 1) / G::BM, tn = (lp + G::BN - 1) / G::BN;
   const int band = 8 * tn, bb = t / band, rr = t - bb * band, h = min(8, tm - bb * 8);
   const int in = rr / h, im = bb * 8 + (rr - in * h);
@@ -289,46 +461,246 @@ __global__ __launch_bounds__(G::NT) void ns_update_kernel(NsGroup g, NsIoGroup i
   G::run(p, x, im * G::BM, in * G::BN, 0, d.s, smem, acc);
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, wm = wid / G::WN, wn = wid % G::WN;
   unsigned short* Y = ws + d.xo + (xbuf ^ 1) * 2 * xplane;
-  const float kp = inv_sp * inv_sx, ka = a * inv_sx;
+  const float kp = st.inv_sp * st.inv_sx, ka = st.a * st.inv_sx;
   float alpha = 0.f;
-  if constexpr (LAST) alpha = io.io[k].alpha * (alpha_dev ? alpha_dev[0] : 1.f);
+  if constexpr (LAST) alpha = io.alpha * (st.alpha_dev ? st.alpha_dev[0] : 1.f);
+  const int mb = im * G::BM + wm * G::TM + (lane & 15), nb = in * G::BN + wn * G::TN + (lane >> 4) * 4;
+  for_rows<G>([&](auto i0, auto rows) {
+    uint2 hh[rows][G::NI], ll[rows][G::NI];
+    load_planes<G, rows>(X, xplane, lp, d.s, lp, mb + i0 * 16, nb, hh, ll);
 #pragma unroll
-  for (int i = 0; i < G::MI; ++i)
+    for (int i = 0; i < rows; ++i)
 #pragma unroll
-    for (int j = 0; j < G::NI; ++j) {
-      const int m = im * G::BM + wm * G::TM + i * 16 + (lane & 15);
-      const int n = in * G::BN + wn * G::TN + j * 16 + (lane >> 4) * 4;
-      if (m >= d.s || n >= lp) continue;
-      const long long o = (long long)m * lp + n;
-      const uint2 hh = *reinterpret_cast<const uint2*>(X + o), ll = *reinterpret_cast<const uint2*>(X + xplane + o);
-      const float xv[4] = {join2(hh.x & 0xffff, ll.x & 0xffff), join2(hh.x >> 16, ll.x >> 16),
-                           join2(hh.y & 0xffff, ll.y & 0xffff), join2(hh.y >> 16, ll.y >> 16)};
-      float v[4];
+      for (int j = 0; j < G::NI; ++j) {
+        const int m = mb + (i0 + i) * 16, n = nb + j * 16;
+        if (m >= d.s || n >= lp) continue;
+        float xv[4], v[4];
+        join4(hh[i][j], ll[i][j], xv);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = fmaf(kp, acc[i][j][e], ka * xv[e]);
-      if constexpr (LAST) {
-        const bool tall = io.io[k].tall;
+        for (int e = 0; e < 4; ++e) v[e] = fmaf(kp, acc[i0 + i][j][e], ka * xv[e]);
+        if constexpr (LAST) {
+          ns_out(io, st.f32, d.s, d.l, m, n, v, alpha, st.beta);
+        } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if (n + e >= d.l) continue;
-          const long long q = tall ? (long long)(n + e) * d.s + m : (long long)m * d.l + n + e;
-          if (f32) {
-            float* dst = static_cast<float*>(io.io[k].dst) + q;
-            *dst = beta != 0.f ? fmaf(alpha, v[e], beta * *dst) : alpha * v[e];
-          } else {
-            bf16_t* dst = static_cast<bf16_t*>(io.io[k].dst) + q;
-            *dst = f2bf(beta != 0.f ? fmaf(alpha, v[e], beta * bf2f(*dst)) : alpha * v[e]);
-          }
+          for (int e = 0; e < 4; ++e) v[e] *= st.so;
+          put_planes(Y, xplane, (long long)m * lp + n, v);
         }
-      } else {
-        unsigned short hi[4], lo[4];
+      }
+  });
+}
+template <class G1, class G2, bool LAST>
+__global__ __launch_bounds__(G1::NT) void ns_update_kernel(const NsTable* __restrict__ tab,
+                                                           unsigned short* __restrict__ ws, int xbuf, NsStep st) {
+  __shared__ __attribute__((aligned(16))) char smem[ns_lds<G1, G2>()];
+  const int L = xcd_remap(blockIdx.x, gridDim.x);
+  const int k = find_matrix(tab, kUpdate, L), t = L - tab->t0[kUpdate][k];
+  const NsDim d = tab->d[k];
+  const NsIo io = LAST ? tab->io[k] : NsIo{};
+  if (tab->b[kUpdate][k].tile == G1::BM) ns_update_tile<G1, LAST>(d, t, io, ws, xbuf, st, smem);
+  else ns_update_tile<G2, LAST>(d, t, io, ws, xbuf, st, smem);
+}
+
+// ------------------------------------------------------------ small matrices
+// A matrix that fits LDS runs all its steps in one block of 16 waves on v_mfma_f32_16x16x4_f32: no
+// launches between the products, and fp32's own precision.  With a shorter side of at most 16 the
+// products run in fp64 (v_mfma_f64_16x16x4_f64): the few singular values share few errors, which then
+// do not average out.  X stays fp32 in LDS.
+// Measured as captured graphs against the many-block kernels: 64 x 27 26 / 62 us, 64 x 64 44 / 76, 16 x 1,000
+// 51 / 85, 64 x 256 81 / 89, 96 x 96 95 / 87, 8 x 4,096 136 / 92 -- the bound on the work keeps the gain, and
+// shorter sides of at most 16 stay here for their accuracy.
+constexpr int kSmallThreads = 1024, kSmallWaves = kSmallThreads / 64;
+constexpr int kSmallElems = 32768;          // s * l: the matrix in at most 136 KiB of LDS
+constexpr int kSmallSide = 96;              // s: S and P beside it
+constexpr long long kSmallWork = 1 << 18;   // s * s * l
+
+typedef __attribute__((ext_vector_type(4))) double f64x4;
+
+template <bool F64>
+struct SmallT {
+  typedef float R;
+  typedef f32x4 Acc;
+  static constexpr int kSplit = kSmallWaves;  // waves that may share a Gram tile
+  static __device__ __forceinline__ Acc mm(R a, R b, Acc c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+  static __device__ __forceinline__ int row(int lane, int e) { return (lane >> 4) * 4 + e; }
+};
+template <>
+struct SmallT<true> {
+  typedef double R;
+  typedef f64x4 Acc;
+  static constexpr int kSplit = kSmallWaves / 2;
+  static __device__ __forceinline__ Acc mm(R a, R b, Acc c) { return __builtin_amdgcn_mfma_f64_16x16x4f64(a, b, c, 0, 0, 0); }
+  static __device__ __forceinline__ int row(int lane, int e) { return e * 4 + (lane >> 4); }
+};
+
+__host__ __device__ inline bool small_f64(int s) { return s <= 16; }
+// row strides: X's a multiple of 64 floats + 4 (the 16 rows x 4 columns of a fragment hit all banks)
+__host__ __device__ inline int small_ldx(int l) { return (l + 63) / 64 * 64 + 4; }
+__host__ __device__ inline int small_lds(int s) { return (s + 15) / 16 * 16 + 4; }
+inline long long small_bytes(int s, int l) {
+  const long long T = (s + 15) / 16, rows = (long long)s * small_ldx(l) * 4;
+  return small_f64(s) ? rows + (2 * 16 * small_lds(s) + SmallT<true>::kSplit * 256) * 8
+                      : rows + (2 * T * 16 * small_lds(s) + SmallT<false>::kSplit * 256) * 4;
+}
+inline bool small_ok(int s, int l) {
+  return s <= kSmallSide && (long long)s * l <= kSmallElems && (small_f64(s) || (long long)s * s * l <= kSmallWork) &&
+         small_bytes(s, l) <= 160 * 1024 - 512;
+}
+
+// one 16 x 16 tile of A B^T over k0 <= k < k1 (multiples of 16): rows m0.. of A, n0.. of B (zero past
+// `rows`), k along the rows
+template <bool F64, typename E>
+__device__ __forceinline__ typename SmallT<F64>::Acc small_dot(const E* M, int ld, int m0, int n0, int rows, int k0,
+                                                               int k1, int lane) {
+  typedef typename SmallT<F64>::R R;
+  const int r = lane & 15, kk = lane >> 4;
+  const bool oka = m0 + r < rows, okb = n0 + r < rows;
+  const E* pa = M + (oka ? m0 + r : 0) * ld + kk;
+  const E* pb = M + (okb ? n0 + r : 0) * ld + kk;
+  typename SmallT<F64>::Acc acc = {0, 0, 0, 0};
+  for (int k = k0; k < k1; k += 16) {
+    E a[4], b[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) split2(v[e] * so, hi[e], lo[e]);
-        *reinterpret_cast<uint2*>(Y + o) = make_uint2(hi[0] | ((uint32_t)hi[1] << 16), hi[2] | ((uint32_t)hi[3] << 16));
-        *reinterpret_cast<uint2*>(Y + xplane + o) =
-            make_uint2(lo[0] | ((uint32_t)lo[1] << 16), lo[2] | ((uint32_t)lo[3] << 16));
+    for (int j = 0; j < 4; ++j) {
+      a[j] = pa[k + 4 * j];
+      b[j] = pb[k + 4 * j];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc = SmallT<F64>::mm((R)(oka ? a[j] : 0), (R)(okb ? b[j] : 0), acc);
+  }
+  return acc;
+}
+
+template <bool F64>
+__device__ __forceinline__ void small_body(const NsDim& dim, const NsIo& o, int f32, int steps, float a, float b,
+                                           float c, float eps, float beta, const float* alpha_dev, char* lds,
+                                           double* red) {
+  typedef SmallT<F64> ST;
+  typedef typename ST::R R;
+  const int s = dim.s, l = dim.l, T = F64 ? 1 : (s + 15) / 16;
+  const int ldx = small_ldx(l), ld = small_lds(s), l16 = (l + 15) & ~15;
+  R* S = reinterpret_cast<R*>(lds);    // [16 T][ld]
+  R* P = S + 16 * T * ld;              // [16 T][ld]
+  R* part = P + 16 * T * ld;           // [kSplit][256]
+  float* X = reinterpret_cast<float*>(part + ST::kSplit * 256);  // [s][ldx], zero past column l
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+  const int n = s * l;
+  for (int i = tid; i < s * (ldx - l); i += kSmallThreads) X[i / (ldx - l) * ldx + l + i % (ldx - l)] = 0.f;
+  double ss = 0.0;
+  for (int i = tid; i < n; i += kSmallThreads) {
+    const float v = ns_ld(o.src, i, f32);
+    const int r = o.tall ? i % s : i / l, q = o.tall ? i / s : i % l;
+    X[r * ldx + q] = v;
+    ss += (double)v * v;
+  }
+  for (int d = 32; d > 0; d >>= 1) ss += __shfl_xor(ss, d, 64);
+  if (lane == 0) red[wid] = ss;
+  __syncthreads();
+  ss = 0.0;
+  for (int w = 0; w < kSmallWaves; ++w) ss += red[w];
+  const double inv = 1.0 / (sqrt(ss) + (double)eps);
+  for (int i = tid; i < s * ldx; i += kSmallThreads) X[i] = (float)(X[i] * inv);
+  const int tiles = T * (T + 1) / 2;
+  const int split = tiles < ST::kSplit ? ST::kSplit / tiles : 1;  // waves that share a Gram tile's sum
+  const int kc = (((l16 + split - 1) / split) + 15) & ~15;
+  for (int step = 0; step < steps; ++step) {
+    __syncthreads();
+    // S = X X^T: lower triangle, then mirrored.  split > 1: partial tiles joined in order
+    for (int u = wid; u < tiles * split; u += kSmallWaves) {
+      const int t = u / split, z = u - t * split;
+      int im, in;
+      tri_of(t, im, in);
+      const typename ST::Acc v = small_dot<F64>(X, ldx, im * 16, in * 16, s, z * kc, min(l16, (z + 1) * kc), lane);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = ST::row(lane, e), q = lane & 15;
+        if (split > 1) {
+          part[u * 256 + r * 16 + q] = v[e];
+        } else {
+          S[(im * 16 + r) * ld + in * 16 + q] = v[e];
+          if (im != in) S[(in * 16 + q) * ld + im * 16 + r] = v[e];
+        }
       }
     }
+    __syncthreads();
+    if (split > 1) {
+      for (int i = tid; i < tiles * 256; i += kSmallThreads) {
+        const int t = i >> 8, r = (i >> 4) & 15, q = i & 15;
+        int im, in;
+        tri_of(t, im, in);
+        R v = 0;
+        for (int z = 0; z < split; ++z) v += part[(t * split + z) * 256 + (i & 255)];
+        S[(im * 16 + r) * ld + in * 16 + q] = v;
+        if (im != in) S[(in * 16 + q) * ld + im * 16 + r] = v;
+      }
+      __syncthreads();
+    }
+    // P = b S + c S S
+    for (int t = wid; t < T * T; t += kSmallWaves) {
+      const int im = t / T, in = t - im * T;
+      const typename ST::Acc v = small_dot<F64>(S, ld, im * 16, in * 16, 16 * T, 0, 16 * T, lane);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int i = (im * 16 + ST::row(lane, e)) * ld + in * 16 + (lane & 15);
+        P[i] = (R)c * v[e] + (R)b * S[i];
+      }
+    }
+    __syncthreads();
+    // X <- a X + P X: a wave owns 16 columns and reads them all before it writes any (P is zero past
+    // row and column s: the rows of X past s are taken as its last one)
+    constexpr int MT = F64 ? 1 : kSmallSide / 16;
+    for (int q0 = wid * 16; q0 < l16; q0 += kSmallWaves * 16) {
+      const int q = q0 + (lane & 15), kk = lane >> 4;
+      typename ST::Acc acc[MT];
+#pragma unroll
+      for (int i = 0; i < MT; ++i) acc[i] = typename ST::Acc{0, 0, 0, 0};
+      for (int r = 0; r < 16 * T; r += 16) {
+        float xb[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) xb[j] = X[min(r + 4 * j + kk, s - 1) * ldx + q];
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+          if (i < T) {
+            R pa[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) pa[j] = P[(i * 16 + (lane & 15)) * ld + r + 4 * j + kk];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[i] = ST::mm(pa[j], (R)xb[j], acc[i]);
+          }
+      }
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+        if (i < T)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int r = i * 16 + ST::row(lane, e);
+            if (r < s) X[r * ldx + q] = (float)((R)a * (R)X[r * ldx + q] + acc[i][e]);
+          }
+    }
+  }
+  __syncthreads();
+  const float alpha = o.alpha * (alpha_dev ? alpha_dev[0] : 1.f);
+  for (int i = tid; i < n; i += kSmallThreads) {
+    const int r = o.tall ? i % s : i / l, q = o.tall ? i / s : i % l;
+    const float v = X[r * ldx + q];
+    if (f32) {
+      float* dst = static_cast<float*>(o.dst) + i;
+      *dst = beta != 0.f ? fmaf(alpha, v, beta * *dst) : alpha * v;
+    } else {
+      bf16_t* dst = static_cast<bf16_t*>(o.dst) + i;
+      *dst = f2bf(beta != 0.f ? fmaf(alpha, v, beta * bf2f(*dst)) : alpha * v);
+    }
+  }
+}
+
+__global__ __launch_bounds__(kSmallThreads) void ns_small_kernel(NsGroup g, int f32, int steps, float a, float b,
+                                                                 float c, float eps, float beta,
+                                                                 const float* __restrict__ alpha_dev) {
+  extern __shared__ __attribute__((aligned(16))) char small_lds_mem[];
+  __shared__ double red[kSmallWaves];
+  const NsDim d = g.d[blockIdx.x];
+  const NsIo io = g.io[blockIdx.x];
+  if (small_f64(d.s)) small_body<true>(d, io, f32, steps, a, b, c, eps, beta, alpha_dev, small_lds_mem, red);
+  else small_body<false>(d, io, f32, steps, a, b, c, eps, beta, alpha_dev, small_lds_mem, red);
 }
 
 // ------------------------------------------------ the optimizer's first pass
@@ -375,86 +747,66 @@ using NsBig = Gemm<256, 256, 2, 4, 32, 2, 2, false, TB, true>;
 template <bool TB>
 using NsMid = Gemm<128, 128, 2, 2, 32, 2, 2, false, TB, true>;
 template <bool TB>
-using NsSmall = Gemm<64, 64, 2, 2, 32, 3, 2, false, TB, true>;
-
+using NsSmall = Gemm<64, 64, 2, 2, 64, 2, 2, false, TB, true>;
+// up to kNsFew blocks, about one a compute unit: eight waves and longer steps, for a block is then bound
+// by the latency of its loads and barriers
+constexpr int kNsFew = 320;
+template <bool TB>
+using NsMidL = Gemm<128, 128, 2, 4, 64, 2, 2, false, TB, true>;
+template <bool TB>
+using NsSmallL = Gemm<64, 64, 2, 4, 64, 4, 2, false, TB, true>;
+// f(G1, G2) with the tiles of a phase of so many blocks
 template <bool TB, typename F>
-void ns_with_tile(int tile, F&& f) {
-  if (tile == 256) f(NsBig<TB>{});
-  else if (tile == 128) f(NsMid<TB>{});
-  else f(NsSmall<TB>{});
+void ns_with(bool latency, F&& f) {
+  if (latency) f(NsMidL<TB>{}, NsSmallL<TB>{});
+  else f(NsMid<TB>{}, NsSmall<TB>{});
 }
 
-inline long long cdiv(long long a, long long b) { return (a + b - 1) / b; }
-inline long long tri(long long t) { return t * (t + 1) / 2; }
-
 struct NsPlan {
-  int gram_tile, poly_tile, upd_tile, kc;
-  NsGroup start, gram, poly, upd;
-  bool slabs;
+  NsCut cut;
+  NsGroup group;
+  int blocks[kPhases], slab_stride;
   long long elems, slab_floats;
 };
 
-// tile of a phase: the largest that gives at least 192 blocks, else the smallest
-template <typename F>
-int ns_pick(const NsMatrix* m, int n, F&& blocks) {
-  for (int t : {256, 128}) {
-    long long b = 0;
-    for (int i = 0; i < n; ++i) b += blocks(m[i], t);
-    if (b >= 192) return t;
-  }
-  return 64;
-}
-
+// Tiles: a 64-wide tile for matrices whose shorter side it covers, else 128 -- unless a phase then has
+// fewer than 128 blocks, which leaves half of the compute units idle: then 64 for all.  The update of
+// large matrices takes 256 where that still fills the device and pads at most 15%.
 NsPlan ns_plan(const NsMatrix* mats, int n) {
   NsPlan p{};
-  auto S = [](const NsMatrix& m) { return std::min(m.rows, m.cols); };
-  auto Lg = [](const NsMatrix& m) { return std::max(m.rows, m.cols); };
-  auto tri_tiles = [&](const NsMatrix& m, int t) { return tri(cdiv(S(m), t)); };
-  auto upd_tiles = [&](const NsMatrix& m, int t) { return cdiv(S(m), t) * cdiv((Lg(m) + 7) / 8 * 8, t); };
-  p.poly_tile = ns_pick(mats, n, tri_tiles);
-  p.upd_tile = ns_pick(mats, n, upd_tiles);
-  // the Gram reduction is cut into pieces of kc, about 512 blocks in all, each at least 256 long
-  p.gram_tile = ns_pick(mats, n, [&](const NsMatrix& m, int t) { return tri_tiles(m, t) * cdiv(Lg(m), 1024); });
-  long long work = 0, longest = 0;
+  long long upd256 = 0, off = 0;
+  int longest = 1;
+  p.group.count = n;
   for (int i = 0; i < n; ++i) {
-    work += tri_tiles(mats[i], p.gram_tile) * Lg(mats[i]);
-    longest = std::max<long long>(longest, Lg(mats[i]));
-  }
-  long long kc = std::max<long long>(256, cdiv(work, 512));
-  p.kc = (int)(std::min(kc, std::max<long long>(longest, 256) + 63) / 64 * 64);
-  long long off = 0, bs = 0, bg = 0, bp = 0, bu = 0;
-  for (int i = 0; i < n; ++i) {
-    NsDim d{};
-    d.s = S(mats[i]);
-    d.l = Lg(mats[i]);
-    const long long lp = (d.l + 7) / 8 * 8, ld = (d.s + 7) / 8 * 8;
+    NsDim& d = p.group.d[i];
+    d.s = std::min(mats[i].rows, mats[i].cols);
+    d.l = std::max(mats[i].rows, mats[i].cols);
     d.xo = off;
-    off += 4 * d.s * lp;
+    off += 4ll * d.s * up8(d.l);
     d.so = off;
-    off += 4 * d.s * ld;
+    off += 4ll * d.s * up8(d.s);
     off = (off + 63) / 64 * 64;
-    d.splits = (int)cdiv(d.l, p.kc);
-    p.slabs = p.slabs || d.splits > 1;
-    d.t0 = (int)bs;
-    p.start.d[i] = d;
-    d.t0 = (int)bg;
-    p.gram.d[i] = d;
-    d.t0 = (int)bp;
-    p.poly.d[i] = d;
-    d.t0 = (int)bu;
-    p.upd.d[i] = d;
-    bs += cdiv(d.s, 64) * cdiv(lp, 64);
-    bg += tri_tiles(mats[i], p.gram_tile) * d.splits;
-    bp += tri_tiles(mats[i], p.poly_tile);
-    bu += upd_tiles(mats[i], p.upd_tile);
+    p.group.io[i] = NsIo{mats[i].src, mats[i].dst, mats[i].alpha, mats[i].rows > mats[i].cols ? 1 : 0};
+    upd256 += cdiv(d.s, 256) * cdiv(up8(d.l), 256);
+    longest = std::max(longest, d.l);
   }
-  p.start.count = p.gram.count = p.poly.count = p.upd.count = n;
-  p.start.blocks = (int)bs;
-  p.gram.blocks = (int)bg;
-  p.poly.blocks = (int)bp;
-  p.upd.blocks = (int)bu;
   p.elems = off;
-  p.slab_floats = p.slabs ? bg * p.gram_tile * p.gram_tile : 0;
+  auto blocks = [&](int phase) {
+    long long b = 0;
+    for (int i = 0; i < n; ++i) b += ns_blocks(phase, p.group.d[i].s, p.group.d[i].l, p.cut).blocks;
+    return b;
+  };
+  p.cut.kc = 256;
+  p.cut.gram_small = blocks(kGram) < 128;
+  p.cut.poly_small = blocks(kPoly) < 128;
+  const long long upd128 = blocks(kUpdate);
+  p.cut.upd_small = upd128 < 128;
+  p.cut.upd_big = upd256 >= 192 && 4 * upd256 * 100 <= upd128 * 115;
+  // the Gram reduction is cut into pieces of kc (at least 256) for about 512 blocks in all
+  while (p.cut.kc < longest && blocks(kGram) > 600) p.cut.kc += 64;
+  for (int ph = 0; ph < kPhases; ++ph) p.blocks[ph] = (int)blocks(ph);
+  p.slab_stride = p.cut.gram_small ? 64 * 64 : 128 * 128;
+  p.slab_floats = p.blocks[kJoin] ? (long long)p.blocks[kGram] * p.slab_stride : 0;
   return p;
 }
 
@@ -489,12 +841,17 @@ bool ns_matrix_ok(const NsMatrix& m) {
   return m.rows >= 1 && m.cols >= 1 && m.rows <= kNsMaxSide && m.cols <= kNsMaxSide;
 }
 
-long long ns_group_bytes(const NsPlan& p, int n, long long* slab_off, long long* part_off) {
-  long long b = (p.elems * 2 + 255) / 256 * 256;
-  *slab_off = b;
-  b += (p.slab_floats * 4 + 255) / 256 * 256;
-  *part_off = b;
-  return b + (long long)n * kNormBlocks * 8;
+struct NsSpace {  // of a group, in bytes
+  long long slab, part, table, total;
+};
+NsSpace ns_space(const NsPlan& p) {
+  auto up = [](long long b) { return (b + 255) / 256 * 256; };
+  NsSpace o;
+  o.slab = up(p.elems * 2);
+  o.part = o.slab + up(p.slab_floats * 4);
+  o.table = o.part + up((long long)p.group.count * kNormBlocks * 8);
+  o.total = o.table + up(sizeof(NsTable));
+  return o;
 }
 
 }  // namespace
@@ -515,12 +872,32 @@ int ns_check(int steps, float a, float b, float c) {
   return ns_scales(steps, a, b, c, sc) ? 0 : 2;
 }
 
-long long ns_workspace_bytes(const NsMatrix* mats, int n) {
-  long long most = 0, so, po;
-  for (int i = 0; i < n; i += kNsGroup) {
-    const int c = std::min(n - i, kNsGroup);
-    most = std::max(most, ns_group_bytes(ns_plan(mats + i, c), c, &so, &po));
+namespace {
+
+// Matrices for the one-block kernel go first; the others in order of their shorter side, the largest
+// first, so that the longest blocks of a grid start first.
+std::vector<NsMatrix> ns_order(const NsMatrix* mats, int n, int* small) {
+  std::vector<NsMatrix> v, rest;
+  for (int i = 0; i < n; ++i) {
+    const int s = std::min(mats[i].rows, mats[i].cols), l = std::max(mats[i].rows, mats[i].cols);
+    (small_ok(s, l) ? v : rest).push_back(mats[i]);
   }
+  *small = (int)v.size();
+  std::stable_sort(rest.begin(), rest.end(), [](const NsMatrix& x, const NsMatrix& y) {
+    return std::min(x.rows, x.cols) > std::min(y.rows, y.cols);
+  });
+  v.insert(v.end(), rest.begin(), rest.end());
+  return v;
+}
+
+}  // namespace
+
+long long ns_workspace_bytes(const NsMatrix* mats, int n) {
+  int small;
+  const std::vector<NsMatrix> v = ns_order(mats, n, &small);
+  long long most = 0;
+  for (int i = small; i < n; i += kNsGroup)
+    most = std::max(most, ns_space(ns_plan(v.data() + i, std::min(n - i, kNsGroup))).total);
   return most;
 }
 
@@ -530,47 +907,57 @@ int ns_launch(const NsMatrix* mats, int n, bool f32, int steps, float a, float b
   if (steps < 1 || steps > kNsMaxSteps || !ns_scales(steps, a, b, c, sc)) return 1;
   for (int i = 0; i < n; ++i)
     if (!ns_matrix_ok(mats[i])) return 2;
-  for (int g0 = 0; g0 < n; g0 += kNsGroup) {
-    const int cnt = std::min(n - g0, kNsGroup);
-    const NsPlan p = ns_plan(mats + g0, cnt);
-    long long slab_off, part_off;
-    ns_group_bytes(p, cnt, &slab_off, &part_off);
+  const int f = f32 ? 1 : 0;
+  int small;
+  const std::vector<NsMatrix> v = ns_order(mats, n, &small);
+  for (int g0 = 0; g0 < small; g0 += kNsGroup) {
+    const NsPlan p = ns_plan(v.data() + g0, std::min(small - g0, kNsGroup));
+    long long bytes = 0;
+    for (int i = 0; i < p.group.count; ++i) bytes = std::max(bytes, small_bytes(p.group.d[i].s, p.group.d[i].l));
+    if (bytes > 64 * 1024 &&
+        hipFuncSetAttribute(reinterpret_cast<const void*>(ns_small_kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                            (int)bytes) != hipSuccess)
+      return 3;
+    hipLaunchKernelGGL(ns_small_kernel, dim3(p.group.count), dim3(kSmallThreads), (size_t)bytes, st, p.group, f, steps, a,
+                       b, c, eps, beta, alpha_dev);
+  }
+  for (int g0 = small; g0 < n; g0 += kNsGroup) {
+    const NsPlan p = ns_plan(v.data() + g0, std::min(n - g0, kNsGroup));
+    const NsSpace o = ns_space(p);
+    char* base = static_cast<char*>(ws);
     unsigned short* W = static_cast<unsigned short*>(ws);
-    float* slab = p.slabs ? reinterpret_cast<float*>(static_cast<char*>(ws) + slab_off) : nullptr;
-    double* part = reinterpret_cast<double*>(static_cast<char*>(ws) + part_off);
-    NsIoGroup io{};
-    for (int i = 0; i < cnt; ++i) {
-      const NsMatrix& m = mats[g0 + i];
-      io.io[i] = NsIo{m.src, m.dst, m.alpha, m.rows > m.cols ? 1 : 0};
-    }
-    const int f = f32 ? 1 : 0;
-    hipLaunchKernelGGL(ns_norm_kernel, dim3(cnt * kNormBlocks), dim3(256), 0, st, p.start, io, f, part);
-    hipLaunchKernelGGL(ns_start_kernel, dim3(p.start.blocks), dim3(256), 0, st, p.start, io, f, part, W, eps, sc[0].x);
+    float* slab = reinterpret_cast<float*>(base + o.slab);
+    double* part = reinterpret_cast<double*>(base + o.part);
+    NsTable* tab = reinterpret_cast<NsTable*>(base + o.table);
+    hipLaunchKernelGGL(ns_norm_kernel, dim3(p.blocks[kNorm]), dim3(256), 0, st, p.group, p.cut, f, part, tab);
+    hipLaunchKernelGGL(ns_start_kernel, dim3(p.blocks[kStart]), dim3(256), 0, st, tab, f, part, W, eps, sc[0].x);
     for (int k = 0; k < steps; ++k) {
       const int xb = k & 1;
       const float gmul = sc[k].s / (sc[k].x * sc[k].x);
-      ns_with_tile<false>(p.gram_tile, [&](auto gm) {
-        using G = decltype(gm);
-        hipLaunchKernelGGL(ns_gram_kernel<G>, dim3(p.gram.blocks), dim3(G::NT), 0, st, p.gram, W, xb, p.kc, gmul,
-                           slab);
-        if (slab)
-          hipLaunchKernelGGL(ns_join_kernel<G::BM>, dim3(p.gram.blocks * 4), dim3(256), 0, st, p.gram, W, slab, gmul);
+      ns_with<false>(p.blocks[kGram] <= kNsFew, [&](auto g1, auto g2) {
+        hipLaunchKernelGGL((ns_gram_kernel<decltype(g1), decltype(g2)>), dim3(p.blocks[kGram]), dim3(g1.NT), 0, st, tab,
+                           W, xb, p.cut.kc, gmul, slab, p.slab_stride);
       });
-      ns_with_tile<false>(p.poly_tile, [&](auto gm) {
-        using G = decltype(gm);
-        hipLaunchKernelGGL(ns_poly_kernel<G>, dim3(p.poly.blocks), dim3(G::NT), 0, st, p.poly, W, b, c, 1.f / sc[k].s,
-                           sc[k].p);
+      if (p.blocks[kJoin])
+        hipLaunchKernelGGL(ns_join_kernel, dim3(p.blocks[kJoin]), dim3(256), 0, st, tab, W, slab, p.slab_stride, gmul);
+      ns_with<false>(p.blocks[kPoly] <= kNsFew, [&](auto g1, auto g2) {
+        hipLaunchKernelGGL((ns_poly_kernel<decltype(g1), decltype(g2)>), dim3(p.blocks[kPoly]), dim3(g1.NT), 0, st, tab,
+                           W, b, c, 1.f / sc[k].s, sc[k].p);
       });
       const bool last = k + 1 == steps;
-      ns_with_tile<true>(p.upd_tile, [&](auto gm) {
-        using G = decltype(gm);
+      const NsStep u{a, 1.f / sc[k].x, 1.f / sc[k].p, last ? 1.f : sc[k + 1].x, beta, f, alpha_dev};
+      auto update = [&](auto g1, auto g2) {
+        using G1 = decltype(g1);
+        using G2 = decltype(g2);
         if (last)
-          hipLaunchKernelGGL((ns_update_kernel<G, true>), dim3(p.upd.blocks), dim3(G::NT), 0, st, p.upd, io, W, xb, a,
-                             1.f / sc[k].x, 1.f / sc[k].p, 1.f, f, beta, alpha_dev);
+          hipLaunchKernelGGL((ns_update_kernel<G1, G2, true>), dim3(p.blocks[kUpdate]), dim3(G1::NT), 0, st, tab, W, xb,
+                             u);
         else
-          hipLaunchKernelGGL((ns_update_kernel<G, false>), dim3(p.upd.blocks), dim3(G::NT), 0, st, p.upd, io, W, xb, a,
-                             1.f / sc[k].x, 1.f / sc[k].p, sc[k + 1].x, f, 0.f, nullptr);
-      });
+          hipLaunchKernelGGL((ns_update_kernel<G1, G2, false>), dim3(p.blocks[kUpdate]), dim3(G1::NT), 0, st, tab, W, xb,
+                             u);
+      };
+      if (p.cut.upd_big) update(NsBig<true>{}, NsBig<true>{});
+      else ns_with<true>(p.blocks[kUpdate] <= kNsFew, update);
     }
   }
   return 0;

@@ -46,7 +46,10 @@ def _check(u, out, full_rank=True, **kw):
 
 
 SIZES = [(1, 1), (1, 9), (7, 1), (2, 3), (64, 27), (64, 147), (63, 65), (128, 64), (65, 576), (200, 130),
-         (512, 128), (257, 1031), (512, 4608), (1000, 2048)]
+         (512, 128), (257, 1031), (512, 4608), (1000, 2048),
+         # at and past the limits of the one-block kernel
+         (96, 96), (97, 97), (96, 113), (96, 114), (101, 96), (32, 1024), (1025, 32), (8, 4096), (4097, 8), (1, 32768),
+         (1, 32769), (17, 1900), (33, 962), (3, 10923)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
