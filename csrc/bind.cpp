@@ -809,26 +809,33 @@ static pmd::GnArgs gn_args(const Tensor& x, const c10::optional<Tensor>& res, co
   return a;
 }
 
-// -> (out, stats [N, G, 2])
+static bool aligned16(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
+
+// -> (out, stats [N, G, 2], mask or None): the mask (training with a residual and ReLU) is what the backward
+// takes in place of the residual
 std::vector<Tensor> group_norm_fwd(Tensor x, c10::optional<Tensor> res, Tensor gamma, Tensor beta, int64_t groups,
-                                   double eps, int64_t act) {
+                                   double eps, int64_t act, bool want_mask) {
   pmd::GnArgs a = gn_args(x, res, gamma, beta, groups, eps, act);
   c10::DeviceGuard g(x.device());
   Tensor out = torch::empty_like(x);
-  Tensor stats = torch::empty({a.N, groups, 2}, gamma.options());
-  if (x.numel() == 0) return {out, stats};
+  Tensor stats = torch::empty({a.N, groups, 2}, gamma.options()), mask;
+  if (x.numel() == 0) return {out, stats, mask};
+  if (want_mask && pmd::gn_wants_mask(a.C, a.esize, a.act, a.res != nullptr) && aligned16(x) && aligned16(*res)) {
+    mask = torch::empty({x.numel() * a.esize / 16}, x.options().dtype(torch::kUInt8));
+    a.mask = mask.data_ptr<uint8_t>();
+  }
   Tensor ws = torch::empty({pmd::gn_fwd_workspace_floats(a.N, a.HW, a.C, a.G, a.esize)}, gamma.options());
   a.stats = stats.data_ptr<float>();
   a.ws = ws.data_ptr<float>();
   a.out = out.data_ptr();
   CHECK_RC(pmd::gn_fwd_launch(a, cur_stream()), "group_norm_fwd");
-  return {out, stats};
+  return {out, stats, mask};
 }
 
-// -> (dx, dres or None); dgamma, dbeta are written (accumulate: added to)
-std::vector<Tensor> group_norm_bwd(Tensor dout, Tensor x, c10::optional<Tensor> res, Tensor gamma, Tensor beta,
-                                   Tensor stats, int64_t groups, int64_t act, Tensor dgamma, Tensor dbeta,
-                                   bool accumulate) {
+// -> (dx, dres or None); dgamma, dbeta are written (accumulate: added to).  With a mask the residual is not read.
+std::vector<Tensor> group_norm_bwd(Tensor dout, Tensor x, c10::optional<Tensor> res, c10::optional<Tensor> mask,
+                                   Tensor gamma, Tensor beta, Tensor stats, int64_t groups, int64_t act,
+                                   bool want_dres, Tensor dgamma, Tensor dbeta, bool accumulate) {
   pmd::GnArgs a = gn_args(x, res, gamma, beta, groups, 0.0, act);
   same_as(dout, x, "group_norm: gradient");
   TORCH_CHECK(stats.device() == x.device() && stats.scalar_type() == torch::kFloat32 && stats.is_contiguous() &&
@@ -838,7 +845,14 @@ std::vector<Tensor> group_norm_bwd(Tensor dout, Tensor x, c10::optional<Tensor> 
   a.accumulate = accumulate;
   c10::DeviceGuard g(x.device());
   Tensor dx = torch::empty_like(x), dres;
-  if (a.res) dres = torch::empty_like(x);
+  if (want_dres) dres = torch::empty_like(x);
+  if (mask && mask->defined()) {
+    TORCH_CHECK(act == 1 && mask->device() == x.device() && mask->scalar_type() == torch::kUInt8 &&
+                mask->is_contiguous() && mask->numel() == x.numel() * a.esize / 16, "group_norm: the forward's mask");
+    a.mask = mask->data_ptr<uint8_t>();
+    a.res = nullptr;
+    if (!aligned16(dout)) dout = dout.clone();  // the mask goes with 16-byte vectors
+  }
   if (x.numel() == 0) {
     if (!accumulate) {
       pmd::zero_launch(dgamma.data_ptr(), dgamma.nbytes(), cur_stream());
@@ -851,7 +865,7 @@ std::vector<Tensor> group_norm_bwd(Tensor dout, Tensor x, c10::optional<Tensor> 
   a.ws = ws.data_ptr<float>();
   a.dout = dout.data_ptr();
   a.dx = dx.data_ptr();
-  a.dres = a.res ? dres.data_ptr() : nullptr;
+  a.dres = want_dres ? dres.data_ptr() : nullptr;
   CHECK_RC(pmd::gn_bwd_launch(a, cur_stream()), "group_norm_bwd");
   return {dx, dres};
 }

@@ -177,15 +177,18 @@ struct GnArgs {
   int N, HW, C, G, act;  // act: 0 none, 1 relu, 2 silu
   float eps;
   const void *x, *res;   // res nullable
+  uint8_t* mask;         // ReLU slopes, one bit per element and a byte per 16-byte vector: written by the
+                         // forward, read by the backward in place of res (nullable; gn_wants_mask)
   const float *gamma, *beta;
   float* stats;          // [N][G][2] mean, rstd: written by the forward, read by the backward
   float* ws;             // gn_*_workspace_floats
   void* out;             // forward
   const void* dout;      // backward
-  void *dx, *dres;       // dres with res
+  void *dx, *dres;       // dres nullable
   float *dgamma, *dbeta;
   bool accumulate;       // dgamma, dbeta += (gradient-arena targets)
 };
+bool gn_wants_mask(int C, int esize, int act, bool res);
 long long gn_fwd_workspace_floats(int N, int HW, int C, int G, int esize);
 long long gn_bwd_workspace_floats(int N, int HW, int C, int G, int esize);
 int gn_fwd_launch(const GnArgs& a, hipStream_t st);

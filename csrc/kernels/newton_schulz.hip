@@ -87,9 +87,8 @@ __host__ __device__ inline NsBlocks ns_blocks(int phase, int s, int l, const NsC
   return b;
 }
 
-// The same in device memory, for the launches that look up their matrix by block: kernel arguments lie
-// in host memory, where a search costs a microsecond a step (a call's 17 launches over one 512 x 4,608
-// matrix took 282 us with the search in the arguments and take 190 us with it here).
+// The same in device memory, written by the first kernel of a call: one load finds a block's matrix, and
+// the later launches carry no descriptions.
 struct NsTable {
   int t0[kPhases][64];  // first block of each matrix (past the last matrix: never reached)
   NsBlocks b[kPhases][kNsGroup];
@@ -122,30 +121,30 @@ __device__ __forceinline__ float join2(unsigned short hi, unsigned short lo) {
 __global__ __launch_bounds__(256) void ns_norm_kernel(NsGroup g, NsCut cut, int f32, double* __restrict__ part,
                                                       NsTable* __restrict__ table) {
   __shared__ double red[4];
-  __shared__ int first[kNsGroup + 1];
-  if (threadIdx.x == 0) {
-    int t = 0;
-    for (int i = 0; i < g.count; ++i) {
-      first[i] = t;
-      t += ns_blocks(kNorm, g.d[i].s, g.d[i].l, cut).blocks;
+  // a lane per matrix (every wave of the block alike): prefix sums of the phases' blocks
+  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+  const bool have = lane < g.count;
+  const int ms = have ? g.d[lane].s : 0, ml = have ? g.d[lane].l : 0;
+  auto first_block = [&](int n) {
+    int t = n;
+    for (int o = 1; o < 64; o <<= 1) {
+      const int v = __shfl_up(t, o, 64);
+      if (lane >= o) t += v;
     }
-    first[g.count] = t;
-  }
-  __syncthreads();
-  int k = 0;
-  while (first[k + 1] <= (int)blockIdx.x) ++k;
-  const int b = blockIdx.x - first[k], nb = first[k + 1] - first[k];
+    return have ? t - n : 0x7fffffff;
+  };
+  const int nb0 = have ? ns_blocks(kNorm, ms, ml, cut).blocks : 0, f0 = first_block(nb0);
+  const int k = 63 - __clzll(__ballot(f0 <= (int)blockIdx.x));
+  const int b = blockIdx.x - __shfl(f0, k, 64), nb = __shfl(nb0, k, 64);
   if (blockIdx.x == 0) {
-    if (threadIdx.x < kPhases) {
-      const int ph = threadIdx.x;
-      int t = 0;
-      for (int i = 0; i < 64; ++i) {
-        table->t0[ph][i] = i < g.count ? t : 0x7fffffff;
-        if (i < g.count) t += (table->b[ph][i] = ns_blocks(ph, g.d[i].s, g.d[i].l, cut)).blocks;
-      }
-    } else if (threadIdx.x >= 64 && threadIdx.x < 64 + g.count) {
-      table->d[threadIdx.x - 64] = g.d[threadIdx.x - 64];
-      table->io[threadIdx.x - 64] = g.io[threadIdx.x - 64];
+    for (int ph = wid; ph < kPhases; ph += 4) {
+      const NsBlocks n = have ? ns_blocks(ph, ms, ml, cut) : NsBlocks{0, 0, 0};
+      table->t0[ph][lane] = first_block(n.blocks);
+      if (have) table->b[ph][lane] = n;
+    }
+    if (have && wid == 3) {
+      table->d[lane] = g.d[lane];
+      table->io[lane] = g.io[lane];
     }
   }
   const long long n = (long long)g.d[k].s * g.d[k].l;
@@ -770,12 +769,13 @@ struct NsPlan {
 };
 
 // Tiles: a 64-wide tile for matrices whose shorter side it covers, else 128 -- unless a phase then has
-// fewer than 128 blocks, which leaves half of the compute units idle: then 64 for all.  The update of
-// large matrices takes 256 where that still fills the device and pads at most 15%.
+// fewer than 128 blocks, which leaves half of the compute units idle: then 64 for all.  The update takes
+// 256 where that still fills the device and no matrix is much narrower (4,096 x 4,096: 335 us on 256, 430 on
+// 128; ResNet-50's mixture: 162 on 256, 144 on 128).
 NsPlan ns_plan(const NsMatrix* mats, int n) {
   NsPlan p{};
   long long upd256 = 0, off = 0;
-  int longest = 1;
+  int longest = 1, shortest = kNsMaxSide;
   p.group.count = n;
   for (int i = 0; i < n; ++i) {
     NsDim& d = p.group.d[i];
@@ -789,6 +789,7 @@ NsPlan ns_plan(const NsMatrix* mats, int n) {
     p.group.io[i] = NsIo{mats[i].src, mats[i].dst, mats[i].alpha, mats[i].rows > mats[i].cols ? 1 : 0};
     upd256 += cdiv(d.s, 256) * cdiv(up8(d.l), 256);
     longest = std::max(longest, d.l);
+    shortest = std::min(shortest, d.s);
   }
   p.elems = off;
   auto blocks = [&](int phase) {
@@ -801,9 +802,10 @@ NsPlan ns_plan(const NsMatrix* mats, int n) {
   p.cut.poly_small = blocks(kPoly) < 128;
   const long long upd128 = blocks(kUpdate);
   p.cut.upd_small = upd128 < 128;
-  p.cut.upd_big = upd256 >= 192 && 4 * upd256 * 100 <= upd128 * 115;
-  // the Gram reduction is cut into pieces of kc (at least 256) for about 512 blocks in all
-  while (p.cut.kc < longest && blocks(kGram) > 600) p.cut.kc += 64;
+  p.cut.upd_big = upd256 >= 192 && shortest > 192;
+  // the Gram reduction is cut into pieces of kc (at least 256), for at most about 1,000 blocks in all
+  // (ResNet-50's mixture: 58 us, and 20 for the join; 68 and 17 with 600 blocks)
+  while (p.cut.kc < longest && blocks(kGram) > 1000) p.cut.kc += 64;
   for (int ph = 0; ph < kPhases; ++ph) p.blocks[ph] = (int)blocks(ph);
   p.slab_stride = p.cut.gram_small ? 64 * 64 : 128 * 128;
   p.slab_floats = p.blocks[kJoin] ? (long long)p.blocks[kGram] * p.slab_stride : 0;

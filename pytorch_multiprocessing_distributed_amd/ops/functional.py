@@ -1530,14 +1530,16 @@ def _param_grads(needs, ps, write):
 
 
 class _GroupNormActFn(torch.autograd.Function):
-    """out = act( GN(x) + res ), one node; saves x (and res) and the [N, G] statistics, and the
-    backward takes the activation's slope from them again."""
+    """out = act( GN(x) + res ), one node; saves x and the [N, G] statistics, from which the backward
+    takes the activation's slope again, and with a residual either ReLU's slopes as bits or it."""
 
     @staticmethod
     def forward(ctx, x, weight, bias, res, groups, eps, act):
         P = prims_for(x)
-        out, stats = P.group_norm_fwd(x, res, weight, bias, groups, eps, act)
-        ctx.save_for_backward(x, res, weight, bias, stats)
+        out, stats, mask = P.group_norm_fwd(x, res, weight, bias, groups, eps, act, any(ctx.needs_input_grad))
+        # act "none" has slope 1: the residual is not needed either
+        keep = None if res is None or mask is not None or act == "none" else res
+        ctx.save_for_backward(x, keep, mask, weight, bias, stats)
         ctx.params = (weight, bias)
         ctx.cfg = (groups, act)
         return out
@@ -1545,16 +1547,16 @@ class _GroupNormActFn(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        x, res, weight, bias, stats = ctx.saved_tensors
+        x, res, mask, weight, bias, stats = ctx.saved_tensors
         groups, act = ctx.cfg
         P = prims_for(x)
         r = []
 
         def write(tgt, accumulate):
-            r.extend(P.group_norm_bwd(dout.contiguous(), x, res, weight, bias, stats, groups, act,
-                                      tgt[0], tgt[1], accumulate))
+            r.extend(P.group_norm_bwd(dout.contiguous(), x, res, mask, weight, bias, stats, groups, act,
+                                      ctx.needs_input_grad[3], tgt[0], tgt[1], accumulate))
         dw, db = _param_grads(ctx.needs_input_grad[1:3], ctx.params, write)
-        return r[0], dw, db, r[1] if ctx.needs_input_grad[3] else None, None, None, None
+        return r[0], dw, db, r[1], None, None, None
 
 
 def group_norm_act(x, gn, residual=None, act="relu"):

@@ -211,16 +211,17 @@ def bn_bwd_elemt_eval(dout, mask, p, relu, want_dzm=False):
 
 
 # --------------------------------------------------------------- group norm
-def group_norm_fwd(x, res, gamma, beta, groups, eps, act):
-    """-> (act(GN(x) + res), stats [N, G, 2] = mean, rstd)."""
+def group_norm_fwd(x, res, gamma, beta, groups, eps, act, want_mask=False):
+    """-> (act(GN(x) + res), stats [N, G, 2] = mean, rstd, mask or None): ``want_mask`` asks for ReLU's
+    slopes as bits, which the backward then takes in place of the residual."""
     return tuple(_C.group_norm_fwd(x, res, gamma.detach(), beta.detach(), int(groups), float(eps),
-                                   _TP.GN_ACTS.index(act)))
+                                   _TP.GN_ACTS.index(act), bool(want_mask)))
 
 
-def group_norm_bwd(dout, x, res, gamma, beta, stats, groups, act, dgamma, dbeta, accumulate):
+def group_norm_bwd(dout, x, res, mask, gamma, beta, stats, groups, act, want_dres, dgamma, dbeta, accumulate):
     """-> (dx, dres or None); dgamma, dbeta (fp32 [C]) are written, or added to."""
-    return tuple(_C.group_norm_bwd(dout, x, res, gamma.detach(), beta.detach(), stats, int(groups),
-                                   _TP.GN_ACTS.index(act), dgamma, dbeta, bool(accumulate)))
+    return tuple(_C.group_norm_bwd(dout, x, res, mask, gamma.detach(), beta.detach(), stats, int(groups),
+                                   _TP.GN_ACTS.index(act), bool(want_dres), dgamma, dbeta, bool(accumulate)))
 
 
 # -------------------------------------------------------------------- pools

@@ -262,11 +262,11 @@ def _gn_z(x, res, gamma, beta, stats, groups):
     return xhat, z
 
 
-def group_norm_fwd(x, res, gamma, beta, groups, eps, act):
-    """-> (act(GN(x) + res), stats [N, G, 2] = mean, rstd) of a channels-last x."""
+def group_norm_fwd(x, res, gamma, beta, groups, eps, act, want_mask=False):
+    """-> (act(GN(x) + res), stats [N, G, 2] = mean, rstd, None) of a channels-last x."""
     n, c = x.shape[0], x.shape[-1]
     if x.numel() == 0:
-        return torch.empty_like(x), torch.zeros(n, groups, 2, dtype=_f(x).dtype, device=x.device)
+        return torch.empty_like(x), torch.zeros(n, groups, 2, dtype=_f(x).dtype, device=x.device), None
     xf = _f(x).reshape(n, -1, groups, c // groups)
     var, mean = torch.var_mean(xf, dim=(1, 3), unbiased=False)
     stats = torch.stack([mean, torch.rsqrt(var + eps)], dim=-1)
@@ -275,10 +275,10 @@ def group_norm_fwd(x, res, gamma, beta, groups, eps, act):
         z = z.clamp_min(0.0)
     elif act == "silu":
         z = z * torch.sigmoid(z)
-    return z.reshape(x.shape).to(x.dtype), stats
+    return z.reshape(x.shape).to(x.dtype), stats, None
 
 
-def group_norm_bwd(dout, x, res, gamma, beta, stats, groups, act, dgamma, dbeta, accumulate):
+def group_norm_bwd(dout, x, res, mask, gamma, beta, stats, groups, act, want_dres, dgamma, dbeta, accumulate):
     """-> (dx, dres or None); dgamma, dbeta are written, or added to."""
     xhat, z = _gn_z(x, res, gamma, beta, stats, groups)
     dz = _f(dout).reshape(z.shape)
@@ -296,7 +296,7 @@ def group_norm_bwd(dout, x, res, gamma, beta, stats, groups, act, dgamma, dbeta,
     dh = dz * _f(gamma.detach()).reshape(groups, -1)
     dx = dh - dh.mean(dim=(1, 3), keepdim=True) - xhat * (dh * xhat).mean(dim=(1, 3), keepdim=True)
     dx = (dx * stats[:, None, :, 1:]).reshape(x.shape).to(x.dtype)
-    return dx, (dz.reshape(x.shape).to(x.dtype) if res is not None else None)
+    return dx, (dz.reshape(x.shape).to(x.dtype) if want_dres else None)
 
 
 # -------------------------------------------------------------------- pools
