@@ -4,6 +4,7 @@
 // kernels do not support (no silent fallback), allocates its outputs through
 // the PyTorch-ROCm caching allocator and launches on the current HIP stream.
 #include <torch/extension.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <pybind11/stl.h>
 #include <c10/hip/HIPStream.h>
 #include <c10/core/DeviceGuard.h>
@@ -871,82 +872,89 @@ std::vector<Tensor> group_norm_bwd(Tensor dout, Tensor x, c10::optional<Tensor> 
 }
 
 // ------------------------------------------------- linear cross-entropy
-static pmd::LxShape lx_shape(const Tensor& x, const Tensor& w, const c10::optional<Tensor>& b, const Tensor& target,
-                             bool bf16_products, pmd::LxIo& io) {
-  CHECK_DEV(x); CHECK_CONT(x); CHECK_CONT(w); CHECK_CONT(target);
-  const bool x16 = act_esize(x, "linear_xent: x") == 2, w16 = act_esize(w, "linear_xent: weight") == 2;
-  TORCH_CHECK(x.dim() == 2 && w.dim() == 2 && x.size(1) == w.size(1), "linear_xent: x [N, D], weight [V, D]");
-  TORCH_CHECK(w.device() == x.device() && target.device() == x.device(),
-              "linear_xent: x, weight and target must be on one device");
-  TORCH_CHECK(target.scalar_type() == torch::kInt64 && target.dim() == 1 && target.size(0) == x.size(0),
+// everything but x itself, which the backward no longer needs
+static pmd::LxShape lx_shape(int64_t N, int64_t D, bool x_f32, const Tensor& w, const c10::optional<Tensor>& b,
+                             const Tensor& target, bool bf16_products, pmd::LxIo& io) {
+  CHECK_DEV(w); CHECK_CONT(w); CHECK_CONT(target);
+  const bool w16 = act_esize(w, "linear_xent: weight") == 2;
+  TORCH_CHECK(w.dim() == 2 && w.size(1) == D, "linear_xent: x [N, D], weight [V, D]");
+  TORCH_CHECK(target.device() == w.device(), "linear_xent: x, weight and target must be on one device");
+  TORCH_CHECK(target.scalar_type() == torch::kInt64 && target.dim() == 1 && target.size(0) == N,
               "linear_xent: target must be int64 [N]");
-  TORCH_CHECK(x.size(0) <= (1 << 24) && w.size(0) >= 1 && w.size(0) <= (1 << 30) && x.size(1) >= 1 &&
-              x.size(1) <= (1 << 21) - 8, "linear_xent: at most 2^24 rows, 2^30 classes, 2^21 - 8 features");
+  TORCH_CHECK(N <= (1 << 24) && w.size(0) >= 1 && w.size(0) <= (1 << 30) && D >= 1 && D <= (1 << 21) - 8,
+              "linear_xent: at most 2^24 rows, 2^30 classes, 2^21 - 8 features");
   pmd::LxShape s{};
-  s.N = (int)x.size(0); s.V = (int)w.size(0); s.D = (int)x.size(1);
-  s.planes = bf16_products || (x16 && w16) ? 1 : 3;
-  s.x_f32 = !x16; s.w_f32 = !w16;
+  s.N = (int)N; s.V = (int)w.size(0); s.D = (int)D;
+  s.planes = bf16_products || (!x_f32 && w16) ? 1 : 3;
+  s.x_f32 = x_f32; s.w_f32 = !w16;
   s.w_aligned = reinterpret_cast<uintptr_t>(w.data_ptr()) % 16 == 0;
-  io.x = x.data_ptr(); io.w = w.data_ptr();
+  io.w = w.data_ptr();
   io.target = reinterpret_cast<const long long*>(target.data_ptr<int64_t>());
   if (b && b->defined()) {
     s.b_f32 = act_esize(*b, "linear_xent: bias") == 4;
-    TORCH_CHECK(b->device() == x.device() && b->is_contiguous() && b->numel() == s.V,
+    TORCH_CHECK(b->device() == w.device() && b->is_contiguous() && b->numel() == s.V,
                 "linear_xent: bias must be [V] on the device of x");
     io.bias = b->data_ptr();
   }
   return s;
 }
 
-// -> (loss [1], correct [1], lse [N], inv_count [1])
+// -> (loss [1], correct [1], lse [N], inv_count [1], xp): the last three are the backward's inputs
 std::vector<Tensor> linear_xent_fwd(Tensor x, Tensor w, c10::optional<Tensor> b, Tensor target, int64_t ignore,
                                     bool bf16_products) {
+  CHECK_DEV(x); CHECK_CONT(x);
+  TORCH_CHECK(x.dim() == 2 && w.device() == x.device(), "linear_xent: x [N, D] and weight must be on one device");
   pmd::LxIo io{};
-  const pmd::LxShape s = lx_shape(x, w, b, target, bf16_products, io);
+  const pmd::LxShape s = lx_shape(x.size(0), x.size(1), act_esize(x, "linear_xent: x") == 4, w, b, target,
+                                  bf16_products, io);
   c10::DeviceGuard g(x.device());
   auto f32 = x.options().dtype(torch::kFloat32);
   Tensor loss = torch::empty({1}, f32), lse = torch::empty({s.N}, f32), inv = torch::empty({1}, f32);
   Tensor correct = torch::empty({1}, x.options().dtype(torch::kInt64));
+  Tensor xp = torch::empty({pmd::lx_xplanes(s)}, x.options().dtype(torch::kBFloat16));
   if (s.N == 0) {
     pmd::zero_launch(loss.data_ptr(), loss.nbytes(), cur_stream());
     pmd::zero_launch(correct.data_ptr(), correct.nbytes(), cur_stream());
-    return {loss, correct, lse, inv};
+    return {loss, correct, lse, inv, xp};
   }
   Tensor ws = torch::empty({pmd::lx_workspace_bytes(s, false)}, x.options().dtype(torch::kUInt8));
+  io.x = x.data_ptr();
   io.ignore = ignore;
   io.ws = ws.data_ptr();
+  io.xp = xp.data_ptr();
   io.loss = loss.data_ptr<float>();
   io.lse = lse.data_ptr<float>();
   io.inv_count = inv.data_ptr<float>();
   io.correct = reinterpret_cast<long long*>(correct.data_ptr<int64_t>());
   CHECK_RC(pmd::lx_fwd_launch(s, io, cur_stream()), "linear_xent_fwd");
-  return {loss, correct, lse, inv};
+  return {loss, correct, lse, inv, xp};
 }
 
-// -> dx (None unless want_dx); dw, db are written, or added to (fp32)
-Tensor linear_xent_bwd(Tensor gloss, Tensor x, Tensor w, c10::optional<Tensor> b, Tensor target, int64_t ignore,
-                       bool bf16_products, Tensor lse, Tensor inv_count, bool want_dx, c10::optional<Tensor> dw,
-                       c10::optional<Tensor> db, bool accumulate) {
+// -> dx [N, D] fp32 or bf16 (None unless want_dx); dw, db are written, or added to (fp32)
+Tensor linear_xent_bwd(Tensor gloss, Tensor xp, bool x_f32, Tensor w, c10::optional<Tensor> b, Tensor target,
+                       int64_t ignore, bool bf16_products, Tensor lse, Tensor inv_count, bool want_dx,
+                       c10::optional<Tensor> dw, c10::optional<Tensor> db, bool accumulate) {
   pmd::LxIo io{};
-  const pmd::LxShape s = lx_shape(x, w, b, target, bf16_products, io);
-  CHECK_F32(gloss); CHECK_F32(lse); CHECK_F32(inv_count); CHECK_CONT(lse);
-  TORCH_CHECK(gloss.device() == x.device() && lse.device() == x.device() && inv_count.device() == x.device() &&
+  const pmd::LxShape s = lx_shape(target.numel(), w.size(-1), x_f32, w, b, target, bf16_products, io);
+  CHECK_F32(gloss); CHECK_F32(lse); CHECK_F32(inv_count); CHECK_CONT(lse); CHECK_CONT(xp);
+  TORCH_CHECK(gloss.device() == w.device() && lse.device() == w.device() && inv_count.device() == w.device() &&
+              xp.device() == w.device() && xp.scalar_type() == torch::kBFloat16 && xp.numel() == pmd::lx_xplanes(s) &&
               gloss.numel() == 1 && inv_count.numel() == 1 && lse.numel() == s.N, "linear_xent: saved tensors");
-  c10::DeviceGuard g(x.device());
+  c10::DeviceGuard g(w.device());
   Tensor dx;
   if (want_dx) {
-    dx = torch::empty_like(x);
+    dx = torch::empty({s.N, s.D}, w.options().dtype(x_f32 ? torch::kFloat32 : torch::kBFloat16));
     io.dx = dx.data_ptr();
   }
   if (dw && dw->defined()) {
-    TORCH_CHECK(dw->device() == x.device() && dw->sizes() == w.sizes() && dw->is_contiguous() &&
+    TORCH_CHECK(dw->device() == w.device() && dw->sizes() == w.sizes() && dw->is_contiguous() &&
                 (dw->scalar_type() == torch::kFloat32 || (dw->scalar_type() == torch::kBFloat16 && !accumulate)),
                 "linear_xent: weight gradient must be [V, D] like the weight (fp32 to accumulate)");
     io.dw = dw->data_ptr();
     io.dw_f32 = dw->scalar_type() == torch::kFloat32;
   }
   if (db && db->defined()) {
-    TORCH_CHECK(io.bias && db->device() == x.device() && db->numel() == s.V && db->is_contiguous() &&
+    TORCH_CHECK(io.bias && db->device() == w.device() && db->numel() == s.V && db->is_contiguous() &&
                 db->scalar_type() == b->scalar_type() && (s.b_f32 || !accumulate),
                 "linear_xent: bias gradient must be [V] like the bias (fp32 to accumulate)");
     io.db = db->data_ptr();
@@ -958,15 +966,109 @@ Tensor linear_xent_bwd(Tensor gloss, Tensor x, Tensor w, c10::optional<Tensor> b
     }
     return dx;
   }
-  Tensor ws = torch::empty({pmd::lx_workspace_bytes(s, true)}, x.options().dtype(torch::kUInt8));
+  Tensor ws = torch::empty({pmd::lx_workspace_bytes(s, true)}, w.options().dtype(torch::kUInt8));
   io.ignore = ignore;
   io.ws = ws.data_ptr();
+  io.xp = xp.data_ptr();
   io.lse = lse.data_ptr<float>();
   io.inv_count = inv_count.data_ptr<float>();
   io.gloss = gloss.data_ptr<float>();
   io.accumulate = accumulate;
   CHECK_RC(pmd::lx_bwd_launch(s, io, cur_stream()), "linear_xent_bwd");
   return dx;
+}
+
+// ---------------------------------------------------- native autograd nodes
+// The same two operators as whole autograd nodes, for parameters that live outside a gradient arena: a
+// Python node costs a small call 25 us more than these (ops/functional.py picks).  As with
+// once_differentiable, gradients of gradients raise.
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+static variable_list once(variable_list g, const char* what) {
+  if (!at::GradMode::is_enabled()) return g;
+  for (Tensor& t : g)
+    if (t.defined()) t = t.detach().set_requires_grad(true);  // else nothing would lead to the error
+  auto err = std::make_shared<torch::autograd::DelayedError>(
+      std::string("trying to differentiate twice through ") + what, (int)g.size());
+  return (*err)(std::move(g));
+}
+
+struct GroupNormActNode : torch::autograd::Function<GroupNormActNode> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const Tensor& bias,
+                        const c10::optional<Tensor>& res, int64_t groups, double eps, int64_t act) {
+    auto r = group_norm_fwd(x, res, weight, bias, groups, eps, act, true);
+    // act 0 has slope 1: the residual is not needed either
+    const bool keep = res && res->defined() && !r[2].defined() && act != 0;
+    ctx->save_for_backward({x, keep ? *res : Tensor(), r[2], weight, bias, r[1]});
+    ctx->saved_data["groups"] = groups;
+    ctx->saved_data["act"] = act;
+    ctx->saved_data["dres"] = res && res->defined() && res->requires_grad();
+    ctx->saved_data["dw"] = weight.requires_grad();
+    ctx->saved_data["db"] = bias.requires_grad();
+    return r[0];
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    auto s = ctx->get_saved_variables();
+    variable_list out(7);
+    {
+      at::AutoGradMode off(false);
+      Tensor dw = torch::empty_like(s[3]), db = torch::empty_like(s[4]);
+      auto r = group_norm_bwd(g[0].contiguous(), s[0], s[1], s[2], s[3], s[4], s[5], ctx->saved_data["groups"].toInt(),
+                              ctx->saved_data["act"].toInt(), ctx->saved_data["dres"].toBool(), dw, db, false);
+      out[0] = r[0];
+      if (ctx->saved_data["dw"].toBool()) out[1] = dw;
+      if (ctx->saved_data["db"].toBool()) out[2] = db;
+      out[3] = r[1];
+    }
+    return once(std::move(out), "group_norm_act");
+  }
+};
+Tensor group_norm_act(Tensor x, Tensor weight, Tensor bias, c10::optional<Tensor> res, int64_t groups, double eps,
+                      int64_t act) {
+  const bool r = res && res->defined() && res->requires_grad();
+  if (!at::GradMode::is_enabled() || !(x.requires_grad() || weight.requires_grad() || bias.requires_grad() || r))
+    return group_norm_fwd(x, res, weight, bias, groups, eps, act, false)[0];
+  return GroupNormActNode::apply(x, weight, bias, res, groups, eps, act);
+}
+
+struct LinearXentNode : torch::autograd::Function<LinearXentNode> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const c10::optional<Tensor>& b,
+                               const Tensor& target, int64_t ignore, bool bf16) {
+    auto r = linear_xent_fwd(x, w, b, target, ignore, bf16);
+    const bool bias = b && b->defined();
+    ctx->save_for_backward({r[4], w, bias ? *b : Tensor(), target, r[2], r[3]});
+    ctx->saved_data["ignore"] = ignore;
+    ctx->saved_data["bf16"] = bf16;
+    ctx->saved_data["x_f32"] = x.scalar_type() == torch::kFloat32;
+    ctx->saved_data["dx"] = x.requires_grad();
+    ctx->saved_data["dw"] = w.requires_grad();
+    ctx->saved_data["db"] = bias && b->requires_grad();
+    ctx->set_materialize_grads(false);
+    Tensor loss = r[0].reshape({});
+    ctx->mark_non_differentiable({r[1]});
+    return {loss, r[1]};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    variable_list out(6);
+    if (!g[0].defined()) return out;
+    auto s = ctx->get_saved_variables();
+    {
+      at::AutoGradMode off(false);
+      Tensor dw, db;
+      if (ctx->saved_data["dw"].toBool()) dw = torch::empty_like(s[1]);
+      if (ctx->saved_data["db"].toBool()) db = torch::empty_like(s[2]);
+      out[0] = linear_xent_bwd(g[0].reshape({1}), s[0], ctx->saved_data["x_f32"].toBool(), s[1], s[2], s[3],
+                               ctx->saved_data["ignore"].toInt(), ctx->saved_data["bf16"].toBool(), s[4], s[5],
+                               ctx->saved_data["dx"].toBool(), dw, db, false);
+      out[1] = dw;
+      out[2] = db;
+    }
+    return once(std::move(out), "linear_cross_entropy");
+  }
+};
+std::vector<Tensor> linear_xent(Tensor x, Tensor w, c10::optional<Tensor> b, Tensor target, int64_t ignore, bool bf16) {
+  return LinearXentNode::apply(x, w, b, target, ignore, bf16);
 }
 
 // ------------------------------------------------------- Newton-Schulz
@@ -1506,6 +1608,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("q8_amax") = py::none(), py::arg("q8_only") = false);
   m.def("group_norm_fwd", &group_norm_fwd);
   m.def("group_norm_bwd", &group_norm_bwd);
+  m.def("group_norm_act", &group_norm_act);
+  m.def("linear_xent", &linear_xent);
   m.def("linear_xent_fwd", &linear_xent_fwd);
   m.def("linear_xent_bwd", &linear_xent_bwd);
   m.def("newton_schulz", &newton_schulz);

@@ -206,12 +206,15 @@ struct LxIo {
   const long long* target;           // [N]
   long long ignore;
   void* ws;                          // lx_workspace_bytes
+  void* xp;                          // lx_xplanes bf16: x laid out, rows to ignore zero; the forward's output,
+                                     // the backward's input (which needs no x)
   float *loss, *lse, *inv_count;     // [1], [N], [1]; lse and inv_count are the backward's inputs
   long long* correct;                // [1]
   const float* gloss;                // backward: d(loss) [1]
   void *dx, *dw, *db;                // nullable; dx in x's type, db in the bias's
   bool dw_f32, accumulate;           // accumulate: dw, db (fp32) +=
 };
+long long lx_xplanes(const LxShape& s);
 long long lx_workspace_bytes(const LxShape& s, bool bwd);
 int lx_fwd_launch(const LxShape& s, const LxIo& io, hipStream_t st);
 int lx_bwd_launch(const LxShape& s, const LxIo& io, hipStream_t st);

@@ -182,23 +182,28 @@ __global__ __launch_bounds__(G::NT) void lx_fwd_kernel(LxArgs<G::PL> a) {
   }
 }
 
-// joins the column tiles of 16 rows a block: lse [N], row loss [N] (0 for rows to ignore), hit [N]
-// (1: kept, 2: kept and top-1 right)
-__global__ __launch_bounds__(256) void lx_combine_kernel(const float* __restrict__ pmax, const float* __restrict__ psum,
-                                                         const int* __restrict__ pidx, const float* __restrict__ tlogit,
-                                                         const long long* __restrict__ target, long long ignore, int N,
-                                                         int V, int tiles, float* __restrict__ lse,
-                                                         float* __restrict__ rloss, int* __restrict__ hit) {
-  __shared__ float sm[16][17], ss[16][17];
-  __shared__ int si[16][17];
-  const int r = threadIdx.x & 15, q = threadIdx.x >> 4, m = blockIdx.x * 16 + r;
+struct LxRows {  // the forward's per-tile results and what joining them gives
+  const float *pmax, *psum, *tlogit;
+  const int* pidx;
+  const long long* target;
+  long long ignore;
+  int N, V, tiles;
+  float *lse, *rloss;  // [N]; the loss of rows to ignore is 0
+  int* hit;            // [N] 0: to ignore, 1: kept, 2: kept and top-1 right
+};
+
+// Joins the column tiles of 16 rows m0..; thread (r, q) of 256 takes every 16th tile of row r.  All threads
+// of the block call this (`t`: the thread's number among its 256).
+__device__ __forceinline__ void lx_join_rows(const LxRows& a, int m0, int t, float (*sm)[17], float (*ss)[17],
+                                             int (*si)[17]) {
+  const int r = t & 15, q = t >> 4, m = m0 + r;
   float mx = -INFINITY, s = 0.f;
   int mi = 0x7fffffff;
-  if (m < N)
-    for (int t = q; t < tiles; t += 16) {
-      const long long o = (long long)t * N + m;
-      const float om = pmax[o], os = psum[o];
-      const int oi = pidx[o];
+  if (m < a.N)
+    for (int c = q; c < a.tiles; c += 16) {
+      const long long o = (long long)c * a.N + m;
+      const float om = a.pmax[o], os = a.psum[o];
+      const int oi = a.pidx[o];
       if (om > mx || (om == mx && oi < mi)) {
         s = (mx == om ? s : s * __expf(mx - om)) + os;  // equal: both may be -inf
         mx = om;
@@ -211,7 +216,7 @@ __global__ __launch_bounds__(256) void lx_combine_kernel(const float* __restrict
   ss[q][r] = s;
   si[q][r] = mi;
   __syncthreads();
-  if (q == 0 && m < N) {
+  if (q == 0 && m < a.N) {
     for (int k = 1; k < 16; ++k)
       if (sm[k][r] > mx || (sm[k][r] == mx && si[k][r] < mi)) {
         mx = sm[k][r];
@@ -220,19 +225,24 @@ __global__ __launch_bounds__(256) void lx_combine_kernel(const float* __restrict
     const float ref = mx == -INFINITY ? 0.f : mx;
     s = 0.f;
     for (int k = 0; k < 16; ++k) s += sm[k][r] == -INFINITY ? ss[k][r] : ss[k][r] * __expf(sm[k][r] - ref);
-    const long long t = target[m];
-    const bool keep = t != ignore, in = t >= 0 && t < V;
+    const long long t0 = a.target[m];
+    const bool keep = t0 != a.ignore, in = t0 >= 0 && t0 < a.V;
     const float l = mx + __logf(s);
-    lse[m] = keep && !in ? NAN : l;
-    rloss[m] = !keep ? 0.f : in ? l - tlogit[m] : NAN;
-    hit[m] = !keep ? 0 : (t == mi ? 2 : 1);
+    a.lse[m] = keep && !in ? NAN : l;
+    a.rloss[m] = !keep ? 0.f : in ? l - a.tlogit[m] : NAN;
+    a.hit[m] = !keep ? 0 : (t0 == mi ? 2 : 1);
   }
 }
 
+__global__ __launch_bounds__(256) void lx_combine_kernel(LxRows a) {
+  __shared__ float sm[16][17], ss[16][17];
+  __shared__ int si[16][17];
+  lx_join_rows(a, blockIdx.x * 16, threadIdx.x, sm, ss, si);
+}
+
 // loss = sum of the row losses / kept, correct, 1 / kept
-__global__ __launch_bounds__(1024) void lx_loss_kernel(const float* __restrict__ rloss, const int* __restrict__ hit,
-                                                       int N, float* __restrict__ loss, long long* __restrict__ correct,
-                                                       float* __restrict__ inv_count) {
+__device__ __forceinline__ void lx_total(const float* rloss, const int* hit, int N, float* loss, long long* correct,
+                                         float* inv_count) {
   __shared__ float sl[16];
   __shared__ int sk[16], sc[16];
   float l = 0.f;
@@ -264,6 +274,24 @@ __global__ __launch_bounds__(1024) void lx_loss_kernel(const float* __restrict__
     correct[0] = c;
     inv_count[0] = 1.f / n;
   }
+}
+__global__ __launch_bounds__(1024) void lx_loss_kernel(const float* __restrict__ rloss, const int* __restrict__ hit,
+                                                       int N, float* __restrict__ loss, long long* __restrict__ correct,
+                                                       float* __restrict__ inv_count) {
+  lx_total(rloss, hit, N, loss, correct, inv_count);
+}
+// both in one block, for few results: 64 rows at a time
+constexpr int kOneBlock = 16384;  // rows x tiles
+__global__ __launch_bounds__(1024) void lx_finish_kernel(LxRows a, float* loss, long long* correct, float* inv_count) {
+  __shared__ float sm[4][16][17], ss[4][16][17];
+  __shared__ int si[4][16][17];
+  const int part = threadIdx.x >> 8;
+  for (int m0 = 0; m0 < a.N; m0 += 64) {
+    lx_join_rows(a, m0 + part * 16, threadIdx.x & 255, sm[part], ss[part], si[part]);
+    __syncthreads();
+  }
+  __threadfence_block();
+  lx_total(a.rloss, a.hit, a.N, loss, correct, inv_count);
 }
 
 // --------------------------------------------------------------- backward
@@ -361,6 +389,21 @@ __device__ __forceinline__ void st4(void* p, bool f32, long long o, const float 
   }
 }
 
+__device__ __forceinline__ void st4v(void* p, bool f32, long long o, const float (&v)[4], bool acc) {
+  if (f32) {
+    float4* d = reinterpret_cast<float4*>(static_cast<float*>(p) + o);
+    float4 t = make_float4(v[0], v[1], v[2], v[3]);
+    if (acc) {
+      const float4 u = *d;
+      t = make_float4(u.x + t.x, u.y + t.y, u.z + t.z, u.w + t.w);
+    }
+    *d = t;
+  } else {
+    *reinterpret_cast<uint2*>(static_cast<bf16_t*>(p) + o) =
+        make_uint2(f2bf(v[0]) | ((uint32_t)f2bf(v[1]) << 16), f2bf(v[2]) | ((uint32_t)f2bf(v[3]) << 16));
+  }
+}
+
 // a gradient product: dst [M][N] = or += scale * A B^T.  ws: split z of the reduction adds to slab z
 // ([splits][M][N] fp32, unscaled) instead.
 template <int PL>
@@ -376,17 +419,17 @@ struct LxGradArgs {
 };
 
 template <class G>
-__global__ __launch_bounds__(G::NT) void lx_grad_kernel(LxGradArgs<G::PL> a) {
-  __shared__ __attribute__((aligned(16))) char smem[G::LDS];
+__device__ __forceinline__ void lx_grad_tile(const LxGradArgs<G::PL>& a, int block, int blocks, int split, char* smem) {
   const int tm = (a.M + G::BM - 1) / G::BM, tn = (a.N + G::BN - 1) / G::BN;
   int im, in;
-  tile_of(blockIdx.x, tm * tn, tm, tn, im, in);
+  tile_of(block, blocks, tm, tn, im, in);
   const int m0 = im * G::BM, n0 = in * G::BN;
-  const int k0 = blockIdx.y * a.ksplit, k1 = min(a.K, k0 + a.ksplit);
+  const int k0 = split * a.ksplit, k1 = min(a.K, k0 + a.ksplit);
   typename G::Acc acc;
   G::run(a.A, a.B, m0, n0, k0, k1, smem, acc);
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, wm = wid / G::WN, wn = wid % G::WN;
   const float sc = a.slab ? 1.f : a.gloss[0] * a.inv_count[0];
+  const bool vec = a.ldd % 4 == 0 && reinterpret_cast<uintptr_t>(a.dst) % 16 == 0;
 #pragma unroll
   for (int i = 0; i < G::MI; ++i) {
     const int m = m0 + wm * G::TM + i * 16 + (lane & 15);
@@ -396,7 +439,7 @@ __global__ __launch_bounds__(G::NT) void lx_grad_kernel(LxGradArgs<G::PL> a) {
       const int n = n0 + wn * G::TN + j * 16 + (lane >> 4) * 4;
       if (n >= a.N) continue;
       if (a.slab) {
-        float* d = a.slab + ((long long)blockIdx.y * a.M + m) * a.N + n;  // N % 8 == 0: whole float4
+        float* d = a.slab + ((long long)split * a.M + m) * a.N + n;  // N % 8 == 0: whole float4
         float4 v = make_float4(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]);
         if (a.slab_add) {
           const float4 o = *reinterpret_cast<const float4*>(d);
@@ -405,28 +448,62 @@ __global__ __launch_bounds__(G::NT) void lx_grad_kernel(LxGradArgs<G::PL> a) {
         *reinterpret_cast<float4*>(d) = v;
       } else {
         const float v[4] = {acc[i][j][0] * sc, acc[i][j][1] * sc, acc[i][j][2] * sc, acc[i][j][3] * sc};
-        st4(a.dst, a.dst_f32, (long long)m * a.ldd + n, v, (int)min(4ll, a.ldd - n), a.accumulate);
+        const long long o = (long long)m * a.ldd + n;
+        if (vec && n + 4 <= a.ldd) st4v(a.dst, a.dst_f32, o, v, a.accumulate);
+        else st4(a.dst, a.dst_f32, o, v, (int)min(4ll, a.ldd - n), a.accumulate);
       }
     }
   }
 }
 
-// dst [M][cols] = scale * sum over the slabs [splits][M][ld]; rows to ignore are zero
-__global__ __launch_bounds__(256) void lx_slab_kernel(const float* __restrict__ slab, int splits, int M, int ld,
-                                                      void* __restrict__ dst, int dst_f32, int cols,
-                                                      const float* __restrict__ gloss,
-                                                      const float* __restrict__ inv_count,
-                                                      const long long* __restrict__ target, long long ignore) {
-  const float sc = gloss[0] * inv_count[0];
-  const int c4 = ld >> 2;
-  const long long total = (long long)M * c4, step = (long long)M * ld;
-  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+// dx (blocks of GX, splits of its reduction one after the other) and dW (GW) in one grid
+template <class GX, class GW>
+__global__ __launch_bounds__(GX::NT) void lx_grads_kernel(LxGradArgs<GX::PL> x, LxGradArgs<GW::PL> w, int xtiles,
+                                                          int xblocks, int wblocks) {
+  __shared__ __attribute__((aligned(16))) char smem[GX::LDS > GW::LDS ? GX::LDS : GW::LDS];
+  const int b = blockIdx.x;
+  if (b < xblocks) lx_grad_tile<GX>(x, b % xtiles, xtiles, b / xtiles, smem);
+  else lx_grad_tile<GW>(w, b - xblocks, wblocks, 0, smem);
+}
+
+// The last kernel of a piece: db [V] = or += scale * column sums of part [tiles][ldp], in blocks of 256
+// classes; and after the last piece dx [M][cols] = scale * sum over the slabs [splits][M][ld] (rows to
+// ignore are zero), in the blocks behind them.
+struct LxTail {
+  const float *part, *slab;
+  void *db, *dx;
+  int tiles, ldp, V, db_f32, accumulate, db_blocks;
+  int splits, M, ld, dx_f32, cols;
+  const float *gloss, *inv_count;
+  const long long* target;
+  long long ignore;
+};
+__global__ __launch_bounds__(256) void lx_tail_kernel(LxTail a) {
+  const float sc = a.gloss[0] * a.inv_count[0];
+  if ((int)blockIdx.x < a.db_blocks) {
+    const int n = blockIdx.x * 256 + threadIdx.x;
+    if (n >= a.V) return;
+    float s = 0.f;
+    for (int t = 0; t < a.tiles; ++t) s += a.part[(long long)t * a.ldp + n];
+    s *= sc;
+    if (a.db_f32) {
+      float* d = static_cast<float*>(a.db) + n;
+      *d = a.accumulate ? *d + s : s;
+    } else {
+      static_cast<bf16_t*>(a.db)[n] = f2bf(s);
+    }
+    return;
+  }
+  const int c4 = a.ld >> 2, blocks = gridDim.x - a.db_blocks;
+  const long long total = (long long)a.M * c4, step = (long long)a.M * a.ld;
+  for (long long i = (blockIdx.x - a.db_blocks) * 256ll + threadIdx.x; i < total; i += blocks * 256ll) {
     const int r = (int)(i / c4), c = (int)(i - (long long)r * c4) * 4;
-    if (c >= cols) continue;
+    if (c >= a.cols) continue;
     float v[4] = {0.f, 0.f, 0.f, 0.f};
-    if (target[r] != ignore) {
-      const float* s = slab + (long long)r * ld + c;
-      for (int z = 0; z < splits; ++z) {
+    if (a.target[r] != a.ignore) {
+      const float* s = a.slab + (long long)r * a.ld + c;
+#pragma unroll 4
+      for (int z = 0; z < a.splits; ++z) {
         const float4 t = *reinterpret_cast<const float4*>(s + z * step);
         v[0] += t.x;
         v[1] += t.y;
@@ -436,25 +513,7 @@ __global__ __launch_bounds__(256) void lx_slab_kernel(const float* __restrict__ 
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] *= sc;
     }
-    st4(dst, dst_f32, (long long)r * cols + c, v, min(4, cols - c), false);
-  }
-}
-
-// db [V] = or += scale * column sums of dbpart [tiles][ldp]
-__global__ __launch_bounds__(256) void lx_db_kernel(const float* __restrict__ part, int tiles, int ldp, int V,
-                                                    void* __restrict__ db, int f32, int accumulate,
-                                                    const float* __restrict__ gloss,
-                                                    const float* __restrict__ inv_count) {
-  const int n = blockIdx.x * 256 + threadIdx.x;
-  if (n >= V) return;
-  float s = 0.f;
-  for (int t = 0; t < tiles; ++t) s += part[(long long)t * ldp + n];
-  s *= gloss[0] * inv_count[0];
-  if (f32) {
-    float* d = static_cast<float*>(db) + n;
-    *d = accumulate ? *d + s : s;
-  } else {
-    static_cast<bf16_t*>(db)[n] = f2bf(s);
+    st4(a.dx, a.dx_f32, (long long)r * a.cols + c, v, min(4, a.cols - c), false);
   }
 }
 
@@ -484,6 +543,19 @@ int with_tile(int tile, F&& f) {
     if (tile == 256) return f(LxBig<TA, TB>{});
   if (tile == 128) return f(typename LxTiles<PL, TA, TB>::Mid{});
   return f(typename LxTiles<PL, TA, TB>::Small{});
+}
+
+// f(tile of dx, tile of dW); the two share a kernel, so a 256-wide one needs the other to be
+template <int PL, typename F>
+void with_tiles(int x, int w, F&& f) {
+  typedef LxTiles<PL, false, true> X;
+  typedef LxTiles<PL, true, true> W;
+  if constexpr (PL == 1)
+    if (x == 256 && w == 256) return f(LxBig<false, true>{}, LxBig<true, true>{});
+  if (x >= 128 && w >= 128) return f(typename X::Mid{}, typename W::Mid{});
+  if (x >= 128) return f(typename X::Mid{}, typename W::Small{});
+  if (w >= 128) return f(typename X::Small{}, typename W::Mid{});
+  return f(typename X::Small{}, typename W::Small{});
 }
 
 inline int grid_cap(long long n, int cap) {
@@ -570,7 +642,7 @@ struct Carver {
 };
 
 struct LxBuf {
-  bf16_t *x, *w;
+  bf16_t *x, *w;  // x: the caller's xp
   float *pmax, *psum, *tlogit, *rloss;
   int *pidx, *hit;
   bf16_t* prob;
@@ -580,7 +652,6 @@ struct LxBuf {
 LxBuf lx_carve(const LxShape& s, const LxPlan& p, bool bwd, char* base, long long* bytes) {
   Carver c{base};
   LxBuf b{};
-  b.x = c.take<bf16_t>((long long)s.planes * s.N * p.Dp);
   if (!p.w_direct) b.w = c.take<bf16_t>((long long)s.planes * s.V * p.Dp);
   if (!bwd) {
     const long long n = (long long)p.fwd_ct * s.N;
@@ -625,7 +696,8 @@ template <int PL>
 int lx_fwd_t(const LxShape& s, const LxIo& io, hipStream_t st) {
   const LxPlan p = lx_plan(s);
   long long bytes;
-  const LxBuf b = lx_carve(s, p, false, static_cast<char*>(io.ws), &bytes);
+  LxBuf b = lx_carve(s, p, false, static_cast<char*>(io.ws), &bytes);
+  b.x = static_cast<bf16_t*>(io.xp);
   lx_prep<PL>(io.x, s.x_f32, s.N, s.D, b.x, p.Dp, io.target, io.ignore, st);
   if (!p.w_direct) lx_prep<PL>(io.w, s.w_f32, s.V, s.D, b.w, p.Dp, nullptr, 0, st);
   LxArgs<PL> a{};
@@ -642,10 +714,14 @@ int lx_fwd_t(const LxShape& s, const LxIo& io, hipStream_t st) {
     return 0;
   });
   if (rc) return rc;
-  hipLaunchKernelGGL(lx_combine_kernel, dim3((s.N + 15) / 16), dim3(256), 0, st, b.pmax, b.psum, b.pidx, b.tlogit,
-                     io.target, io.ignore, s.N, s.V, p.fwd_ct, io.lse, b.rloss, b.hit);
-  hipLaunchKernelGGL(lx_loss_kernel, dim3(1), dim3(1024), 0, st, b.rloss, b.hit, s.N, io.loss, io.correct,
-                     io.inv_count);
+  const LxRows r{b.pmax, b.psum, b.tlogit, b.pidx, io.target, io.ignore, s.N, s.V, p.fwd_ct, io.lse, b.rloss, b.hit};
+  if ((long long)s.N * p.fwd_ct <= kOneBlock) {
+    hipLaunchKernelGGL(lx_finish_kernel, dim3(1), dim3(1024), 0, st, r, io.loss, io.correct, io.inv_count);
+  } else {
+    hipLaunchKernelGGL(lx_combine_kernel, dim3((s.N + 15) / 16), dim3(256), 0, st, r);
+    hipLaunchKernelGGL(lx_loss_kernel, dim3(1), dim3(1024), 0, st, b.rloss, b.hit, s.N, io.loss, io.correct,
+                       io.inv_count);
+  }
   return 0;
 }
 
@@ -653,8 +729,8 @@ template <int PL>
 int lx_bwd_t(const LxShape& s, const LxIo& io, hipStream_t st) {
   const LxPlan p = lx_plan(s);
   long long bytes;
-  const LxBuf b = lx_carve(s, p, true, static_cast<char*>(io.ws), &bytes);
-  lx_prep<PL>(io.x, s.x_f32, s.N, s.D, b.x, p.Dp, io.target, io.ignore, st);
+  LxBuf b = lx_carve(s, p, true, static_cast<char*>(io.ws), &bytes);
+  b.x = static_cast<bf16_t*>(io.xp);  // the forward's
   if (!p.w_direct) lx_prep<PL>(io.w, s.w_f32, s.V, s.D, b.w, p.Dp, nullptr, 0, st);
   const bf16_t* wbase = p.w_direct ? static_cast<const bf16_t*>(io.w) : b.w;
   const long long wplane = p.w_direct ? 0 : (long long)s.V * p.Dp;
@@ -676,47 +752,61 @@ int lx_bwd_t(const LxShape& s, const LxIo& io, hipStream_t st) {
       hipLaunchKernelGGL(lx_prob_kernel<G>, dim3((unsigned)tiles_of(s.N, a.ldp, G::BM)), dim3(G::NT), 0, st, a);
       return 0;
     });
-    if (io.db)
-      hipLaunchKernelGGL(lx_db_kernel, dim3((V + 255) / 256), dim3(256), 0, st, b.dbpart, p.bwd_rt, a.ldp, V,
-                         static_cast<void*>(static_cast<char*>(io.db) + (long long)v0 * (s.b_f32 ? 4 : 2)),
-                         s.b_f32 ? 1 : 0, io.accumulate ? 1 : 0, io.gloss, io.inv_count);
+    LxGradArgs<PL> x{}, w{};
     if (io.dx) {  // slabs [splits][N][Dp] += prob W
-      LxGradArgs<PL> d{};
-      d.A = planes_of<PL>(b.prob, a.pplane, a.ldp, s.N);
-      d.B = planes_of<PL>(wbase + (long long)v0 * p.Dp, wplane, p.Dp, p.Dp);
-      d.M = s.N; d.N = p.Dp; d.K = V; d.ksplit = p.dx_ksplit;
-      d.slab = b.slab; d.slab_add = k > 0;
-      with_tile<PL, false, true>(p.dx_tile, [&](auto g) {
-        using G = decltype(g);
-        hipLaunchKernelGGL(lx_grad_kernel<G>, dim3((unsigned)tiles_of(s.N, p.Dp, G::BM), p.dx_splits), dim3(G::NT), 0,
-                           st, d);
-        return 0;
-      });
+      x.A = planes_of<PL>(b.prob, a.pplane, a.ldp, s.N);
+      x.B = planes_of<PL>(wbase + (long long)v0 * p.Dp, wplane, p.Dp, p.Dp);
+      x.M = s.N; x.N = p.Dp; x.K = V; x.ksplit = p.dx_ksplit;
+      x.slab = b.slab; x.slab_add = k > 0;
     }
     if (io.dw) {  // dW[v0 ..] = or += scale prob^T x
-      LxGradArgs<PL> d{};
-      d.A = planes_of<PL>(b.prob, a.pplane, a.ldp, a.ldp);
-      d.B = planes_of<PL>(b.x, (long long)s.N * p.Dp, p.Dp, p.Dp);
-      d.M = V; d.N = p.Dp; d.K = s.N; d.ksplit = up(s.N, 64);
-      d.dst = static_cast<char*>(io.dw) + (long long)v0 * s.D * (io.dw_f32 ? 4 : 2);
-      d.ldd = s.D; d.dst_f32 = io.dw_f32; d.accumulate = io.accumulate;
-      d.gloss = io.gloss; d.inv_count = io.inv_count;
-      with_tile<PL, true, true>(p.dw_tile, [&](auto g) {
-        using G = decltype(g);
-        hipLaunchKernelGGL(lx_grad_kernel<G>, dim3((unsigned)tiles_of(V, p.Dp, G::BM)), dim3(G::NT), 0, st, d);
-        return 0;
-      });
+      w.A = planes_of<PL>(b.prob, a.pplane, a.ldp, a.ldp);
+      w.B = planes_of<PL>(b.x, (long long)s.N * p.Dp, p.Dp, p.Dp);
+      w.M = V; w.N = p.Dp; w.K = s.N; w.ksplit = up(s.N, 64);
+      w.dst = static_cast<char*>(io.dw) + (long long)v0 * s.D * (io.dw_f32 ? 4 : 2);
+      w.ldd = s.D; w.dst_f32 = io.dw_f32; w.accumulate = io.accumulate;
+      w.gloss = io.gloss; w.inv_count = io.inv_count;
     }
-  }
-  if (io.dx) {
-    const long long n = (long long)s.N * (p.Dp / 4);
-    hipLaunchKernelGGL(lx_slab_kernel, dim3(grid_cap((n + 255) / 256, 4096)), dim3(256), 0, st, b.slab, p.dx_splits,
-                       s.N, p.Dp, io.dx, s.x_f32 ? 1 : 0, s.D, io.gloss, io.inv_count, io.target, io.ignore);
+    if (io.dx || io.dw) with_tiles<PL>(p.dx_tile, p.dw_tile, [&](auto gx, auto gw) {
+      using GX = decltype(gx);
+      using GW = decltype(gw);
+      const int xt = io.dx ? (int)tiles_of(s.N, p.Dp, GX::BM) : 1, xb = io.dx ? xt * p.dx_splits : 0;
+      const int wb = io.dw ? (int)tiles_of(V, p.Dp, GW::BM) : 0;
+      auto launch = [&](int xblocks, int wblocks) {
+        hipLaunchKernelGGL((lx_grads_kernel<GX, GW>), dim3((unsigned)(xblocks + wblocks)), dim3(GX::NT), 0, st, x, w, xt,
+                           xblocks, wblocks);
+      };
+      // one grid where a product alone leaves compute units idle; two where each has rounds of its own
+      if (xb < 256 || wb < 256) {
+        launch(xb, wb);
+      } else {
+        launch(xb, 0);
+        launch(0, wb);
+      }
+    });
+    const bool last = k + 1 == p.pieces;
+    if (io.db || (last && io.dx)) {
+      LxTail t{};
+      t.gloss = io.gloss; t.inv_count = io.inv_count; t.target = io.target; t.ignore = io.ignore;
+      if (io.db) {
+        t.part = b.dbpart; t.tiles = p.bwd_rt; t.ldp = a.ldp; t.V = V;
+        t.db = static_cast<char*>(io.db) + (long long)v0 * bsz; t.db_f32 = s.b_f32; t.accumulate = io.accumulate;
+        t.db_blocks = (V + 255) / 256;
+      }
+      long long nb = 0;
+      if (last && io.dx) {
+        t.slab = b.slab; t.splits = p.dx_splits; t.M = s.N; t.ld = p.Dp; t.dx = io.dx; t.dx_f32 = s.x_f32; t.cols = s.D;
+        nb = grid_cap(((long long)s.N * (p.Dp / 4) + 255) / 256, 4096);
+      }
+      hipLaunchKernelGGL(lx_tail_kernel, dim3((unsigned)(t.db_blocks + nb)), dim3(256), 0, st, t);
+    }
   }
   return 0;
 }
 
 }  // namespace
+
+long long lx_xplanes(const LxShape& s) { return (long long)s.planes * s.N * up(s.D, 8); }
 
 long long lx_workspace_bytes(const LxShape& s, bool bwd) {
   if (!lx_ok(s)) return 0;

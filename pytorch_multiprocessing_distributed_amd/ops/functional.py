@@ -1515,6 +1515,13 @@ def residual_block(x, stages, final, shortcut, training):
 
 
 # ---------------------------------------------------------------- group norm
+def _native_node(x, *params):
+    """Whether an operator on ``x`` runs as the extension's own autograd node: on the GPU, with no
+    parameter in a gradient arena (those gradients are written in place and reported from Python)."""
+    return (x.is_cuda and not _state["force_torch"]
+            and not any(p is not None and getattr(p, "_pmd_direct", False) for p in params))
+
+
 def _param_grads(needs, ps, write):
     """Gradients of the parameters ``ps`` by ``write(targets, accumulate)``: added to their arena
     views when all live there (then reported ready, and None is returned for each), else written to
@@ -1581,8 +1588,10 @@ def group_norm_act(x, gn, residual=None, act="relu"):
             raise ValueError(f"residual must be {tuple(x.shape)} {x.dtype}, got "
                              f"{tuple(residual.shape)} {residual.dtype}")
         residual = residual.contiguous()
-    return _GroupNormActFn.apply(x.contiguous(), gn.weight, gn.bias, residual, int(gn.num_groups),
-                                 float(gn.eps), act)
+    args = (x.contiguous(), gn.weight, gn.bias, residual, int(gn.num_groups), float(gn.eps), act)
+    if _native_node(x, gn.weight, gn.bias):
+        return prims_for(x).group_norm_act(*args)
+    return _GroupNormActFn.apply(*args)
 
 
 # --------------------------------------------------------------------- pools
@@ -1691,10 +1700,10 @@ class _LinearXentFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, b, target, ignore, bf16):
         P = prims_for(x)
-        loss, correct, lse, inv = P.linear_xent_fwd(x, w, b, target, ignore, bf16)
-        ctx.save_for_backward(x, w, b, target, lse, inv)
+        loss, correct, lse, inv, xp = P.linear_xent_fwd(x, w, b, target, ignore, bf16)
+        ctx.save_for_backward(xp, w, b, target, lse, inv)
         ctx.params = (w, b)
-        ctx.cfg = (ignore, bf16)
+        ctx.cfg = (ignore, bf16, x.dtype)
         ctx.mark_non_differentiable(correct)
         ctx.set_materialize_grads(False)
         return loss.reshape(()), correct
@@ -1704,10 +1713,10 @@ class _LinearXentFn(torch.autograd.Function):
     def backward(ctx, gloss, _gcorrect):
         if gloss is None:
             return (None,) * 6
-        x, w, b, target, lse, inv = ctx.saved_tensors
+        xp, w, b, target, lse, inv = ctx.saved_tensors
         wp, bp = ctx.params
-        ignore, bf16 = ctx.cfg
-        P = prims_for(x)
+        ignore, bf16, x_dtype = ctx.cfg
+        P = prims_for(w)
         tw = _grad_target(wp)
         tb = _grad_target(bp) if bp is not None else None
         arena = tw is not None and (bp is None or tb is not None)
@@ -1720,7 +1729,8 @@ class _LinearXentFn(torch.autograd.Function):
             if b is not None and ctx.needs_input_grad[2]:
                 db = torch.empty_like(b)
         g = gloss.reshape(1).to(lse.dtype)
-        dx = P.linear_xent_bwd(g, x, w, b, target, ignore, bf16, lse, inv, ctx.needs_input_grad[0], dw, db, arena)
+        dx = P.linear_xent_bwd(g, xp, x_dtype, w, b, target, ignore, bf16, lse, inv, ctx.needs_input_grad[0], dw, db,
+                               arena)
         if arena:
             _ready(wp, *([bp] if bp is not None else []))
             dw = db = None
@@ -1751,9 +1761,11 @@ def linear_cross_entropy(x, lin, target, ignore_index=-100, compute_dtype=None):
         raise ValueError(f"target must be {tuple(x.shape[:-1])}, got {tuple(target.shape)}")
     if target.dtype != torch.int64:
         raise ValueError(f"target must be int64 class indices, got {target.dtype}")
-    return _LinearXentFn.apply(x.reshape(-1, x.shape[-1]).contiguous(), w.contiguous(), b,
-                               target.reshape(-1).contiguous(), int(ignore_index),
-                               compute_dtype is not None)
+    args = (x.reshape(-1, x.shape[-1]).contiguous(), w.contiguous(), b, target.reshape(-1).contiguous(),
+            int(ignore_index), compute_dtype is not None)
+    if _native_node(x, w, b):
+        return prims_for(x).linear_xent(*args)
+    return _LinearXentFn.apply(*args)
 
 
 _SEEDS: dict = {}

@@ -295,15 +295,26 @@ def xent_bwd(gloss, logits, target, lse):
 
 
 def linear_xent_fwd(x, w, b, target, ignore, bf16):
-    """-> (loss [1], correct [1], lse [N], 1 / kept rows [1]); no logits are stored."""
+    """-> (loss [1], correct [1], and for the backward: lse [N], 1 / kept rows [1], x laid out); no logits
+    are stored."""
     return tuple(_C.linear_xent_fwd(x, w.detach(), None if b is None else b.detach(), target, int(ignore),
                                     bool(bf16)))
 
 
-def linear_xent_bwd(gloss, x, w, b, target, ignore, bf16, lse, inv_count, want_dx, dw, db, accumulate):
+def linear_xent_bwd(gloss, xp, x_dtype, w, b, target, ignore, bf16, lse, inv_count, want_dx, dw, db, accumulate):
     """-> dx or None; ``dw`` / ``db`` (None: not wanted) are written, or added to (fp32 targets)."""
-    return _C.linear_xent_bwd(gloss, x, w.detach(), None if b is None else b.detach(), target, int(ignore),
-                              bool(bf16), lse, inv_count, bool(want_dx), dw, db, bool(accumulate))
+    return _C.linear_xent_bwd(gloss, xp, x_dtype == torch.float32, w.detach(), None if b is None else b.detach(),
+                              target, int(ignore), bool(bf16), lse, inv_count, bool(want_dx), dw, db, bool(accumulate))
+
+
+def group_norm_act(x, weight, bias, res, groups, eps, act):
+    """The whole operator as a native autograd node."""
+    return _C.group_norm_act(x, weight, bias, res, groups, eps, _TP.GN_ACTS.index(act))
+
+
+def linear_xent(x, w, b, target, ignore, bf16):
+    """(loss, correct): the whole operator as a native autograd node."""
+    return tuple(_C.linear_xent(x, w, b, target, ignore, bf16))
 
 
 def correct_count(logits, target):

@@ -394,7 +394,7 @@ def _lx_operands(x, w, b, bf16):
 
 def linear_xent_fwd(x, w, b, target, ignore, bf16):
     """Mean softmax cross-entropy of ``x w^T + b`` over the rows whose target is not ``ignore``:
-    (loss [1], top-1 count [1], lse [N], 1 / kept rows [1]).  No row kept: loss 0.  A target outside
+    (loss [1], top-1 count [1], lse [N], 1 / kept rows [1], x).  No row kept: loss 0.  A target outside
     the classes makes its row's loss NaN."""
     xf, wf, bf = _lx_operands(x, w, b, bf16)
     keep = target != ignore
@@ -409,10 +409,10 @@ def linear_xent_fwd(x, w, b, target, ignore, bf16):
     correct = torch.zeros(1, dtype=torch.int64, device=x.device)
     if x.shape[0]:
         correct = ((logits.argmax(1) == target) & keep).sum().reshape(1)
-    return rows.sum().reshape(1) * inv, correct, torch.where(keep & ~valid, nan, lse), inv
+    return rows.sum().reshape(1) * inv, correct, torch.where(keep & ~valid, nan, lse), inv, x
 
 
-def linear_xent_bwd(gloss, x, w, b, target, ignore, bf16, lse, inv_count, want_dx, dw, db, accumulate):
+def linear_xent_bwd(gloss, x, x_dtype, w, b, target, ignore, bf16, lse, inv_count, want_dx, dw, db, accumulate):
     """-> dx or None; ``dw`` / ``db`` (None: not wanted) are written, or added to."""
     xf, wf, bf = _lx_operands(x, w, b, bf16)
     keep = target != ignore
@@ -424,7 +424,7 @@ def linear_xent_bwd(gloss, x, w, b, target, ignore, bf16, lse, inv_count, want_d
     for tgt, g in ((dw, lambda: p.t() @ xf), (db, lambda: p.sum(0))):
         if tgt is not None:
             tgt.add_(g().to(tgt.dtype)) if accumulate else tgt.copy_(g())
-    return torch.where(keep[:, None], p @ wf, torch.zeros_like(xf)).to(x.dtype) if want_dx else None
+    return torch.where(keep[:, None], p @ wf, torch.zeros_like(xf)).to(x_dtype) if want_dx else None
 
 
 def correct_count(logits, target):

@@ -211,3 +211,42 @@ def test_refusals_gpu():
     big = torch.nn.GroupNorm(1, 16392).cuda()
     with pytest.raises(RuntimeError, match="channels"):
         OF.group_norm_act(torch.zeros(1, 16392, device="cuda"), big)
+
+
+@pytest.mark.parametrize("act", ["none", "relu", "silu"])
+def test_native_and_python_nodes_agree(act):
+    x, gn, res, dy = _case(2, (6, 6), 32, 8, torch.bfloat16, seed=10)
+
+    def grads(fn):
+        xg, rg = x.clone().requires_grad_(True), res.clone().requires_grad_(True)
+        out = fn(xg, rg)
+        return [out.detach(), *torch.autograd.grad(out, [xg, rg, gn.weight, gn.bias], dy)]
+    a = grads(lambda xg, rg: OF.group_norm_act(xg, gn, residual=rg, act=act))
+    b = grads(lambda xg, rg: OF._GroupNormActFn.apply(xg, gn.weight, gn.bias, rg, 8, gn.eps, act))
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def test_frozen_inputs_and_no_second_derivative():
+    x, gn, res, dy = _case(2, (6, 6), 32, 8, torch.float32, seed=11)
+    gn.weight.requires_grad_(False)
+    out = OF.group_norm_act(x, gn, residual=res)                    # only the bias wants a gradient
+    (gb,) = torch.autograd.grad(out, gn.bias, dy)
+    assert (gb.double() - (dy.double() * (out > 0)).sum((0, 1, 2))).abs().max() <= 512 * U32 * dy.abs().sum((0, 1, 2)).max()
+    assert not OF.group_norm_act(x, gn.requires_grad_(False), residual=res).requires_grad
+    xg = x.clone().requires_grad_(True)
+    (gx,) = torch.autograd.grad(OF.group_norm_act(xg, gn).sum(), xg, create_graph=True)
+    with pytest.raises(RuntimeError):                # nothing leads from the gradient back to the input
+        torch.autograd.grad(gx.sum(), xg, retain_graph=True)
+    with pytest.raises(RuntimeError, match="twice"):
+        gx.sum().backward()
+
+
+def test_misaligned_gradient_with_the_mask():
+    x, gn, res, dy = _case(2, (6, 6), 64, 8, torch.bfloat16, seed=12)
+    buf = torch.empty(dy.numel() + 8, dtype=dy.dtype, device="cuda")
+    off = buf[1:1 + dy.numel()].view(dy.shape)
+    off.copy_(dy)
+    xg = x.clone().requires_grad_(True)
+    out = OF.group_norm_act(xg, gn, residual=res)
+    a, b = torch.autograd.grad(out, xg, dy, retain_graph=True), torch.autograd.grad(out, xg, off)
+    assert torch.equal(a[0], b[0])

@@ -273,3 +273,39 @@ def test_refusals_gpu():
         OF.linear_cross_entropy(x, lin, t.cpu())
     with pytest.raises(RuntimeError, match="one device"):
         OF.linear_cross_entropy(x, torch.nn.Linear(8, 6), t)
+
+
+def test_native_and_python_nodes_agree():
+    x, lin, t = _case(70, 96, 333, torch.bfloat16, seed=14)
+
+    def grads(fn):
+        loss, c = fn()
+        return [loss.detach(), c, *torch.autograd.grad(loss, [x, lin.weight, lin.bias], torch.tensor(0.5, device="cuda"))]
+    a = grads(lambda: OF.linear_cross_entropy(x, lin, t))
+    b = grads(lambda: OF._LinearXentFn.apply(x, lin.weight, lin.bias, t, -100, False))
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def test_frozen_inputs_and_no_second_derivative():
+    x, lin, t = _case(70, 96, 333, torch.bfloat16, seed=15)
+    loss, _ = OF.linear_cross_entropy(x, lin, t)
+    all_of = torch.autograd.grad(loss, [x, lin.weight, lin.bias])
+    lin.weight.requires_grad_(False)
+    loss, _ = OF.linear_cross_entropy(x, lin, t)
+    gx, gb = torch.autograd.grad(loss, [x, lin.bias])
+    assert torch.equal(gx, all_of[0]) and torch.equal(gb, all_of[2])
+    lin.weight.requires_grad_(True)
+    loss, _ = OF.linear_cross_entropy(x.detach(), lin, t)
+    (gw,) = torch.autograd.grad(loss, [lin.weight])
+    assert torch.equal(gw, all_of[1])
+    (gx,) = torch.autograd.grad(OF.linear_cross_entropy(x, lin, t)[0], x, create_graph=True)
+    with pytest.raises(RuntimeError):                # nothing leads from the gradient back to the input
+        torch.autograd.grad(gx.sum(), x, retain_graph=True)
+    with pytest.raises(RuntimeError, match="twice"):
+        gx.sum().backward()
+
+
+def test_two_products_that_fill_the_device_alone():
+    # dx and dW of 256 blocks and more each take a grid of their own
+    x, lin, t = _case(1100, 2064, 9001, torch.bfloat16, seed=16)
+    _check(x, lin, t)
