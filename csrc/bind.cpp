@@ -899,9 +899,10 @@ static pmd::LxShape lx_shape(int64_t N, int64_t D, bool x_f32, const Tensor& w, 
   return s;
 }
 
-// -> (loss [1], correct [1], lse [N], inv_count [1], xp): the last three are the backward's inputs
+// -> (loss [1], correct [1], lse [N], inv_count [1], xp, kept): the last four are the backward's inputs; kept
+// is empty unless a backward will follow and what it needs is small enough
 std::vector<Tensor> linear_xent_fwd(Tensor x, Tensor w, c10::optional<Tensor> b, Tensor target, int64_t ignore,
-                                    bool bf16_products) {
+                                    bool bf16_products, bool want_grad) {
   CHECK_DEV(x); CHECK_CONT(x);
   TORCH_CHECK(x.dim() == 2 && w.device() == x.device(), "linear_xent: x [N, D] and weight must be on one device");
   pmd::LxIo io{};
@@ -912,12 +913,16 @@ std::vector<Tensor> linear_xent_fwd(Tensor x, Tensor w, c10::optional<Tensor> b,
   Tensor loss = torch::empty({1}, f32), lse = torch::empty({s.N}, f32), inv = torch::empty({1}, f32);
   Tensor correct = torch::empty({1}, x.options().dtype(torch::kInt64));
   Tensor xp = torch::empty({pmd::lx_xplanes(s)}, x.options().dtype(torch::kBFloat16));
+  auto u8 = x.options().dtype(torch::kUInt8);
+  const long long kb = want_grad && s.N ? pmd::lx_kept_bytes(s) : 0;
+  Tensor kept = torch::empty({kb}, u8);
   if (s.N == 0) {
     pmd::zero_launch(loss.data_ptr(), loss.nbytes(), cur_stream());
     pmd::zero_launch(correct.data_ptr(), correct.nbytes(), cur_stream());
-    return {loss, correct, lse, inv, xp};
+    return {loss, correct, lse, inv, xp, kept};
   }
-  Tensor ws = torch::empty({pmd::lx_workspace_bytes(s, false)}, x.options().dtype(torch::kUInt8));
+  Tensor ws = torch::empty({pmd::lx_workspace_bytes(s, false, kb > 0)}, u8);
+  if (kb) io.kept = kept.data_ptr();
   io.x = x.data_ptr();
   io.ignore = ignore;
   io.ws = ws.data_ptr();
@@ -927,19 +932,21 @@ std::vector<Tensor> linear_xent_fwd(Tensor x, Tensor w, c10::optional<Tensor> b,
   io.inv_count = inv.data_ptr<float>();
   io.correct = reinterpret_cast<long long*>(correct.data_ptr<int64_t>());
   CHECK_RC(pmd::lx_fwd_launch(s, io, cur_stream()), "linear_xent_fwd");
-  return {loss, correct, lse, inv, xp};
+  return {loss, correct, lse, inv, xp, kept};
 }
 
 // -> dx [N, D] fp32 or bf16 (None unless want_dx); dw, db are written, or added to (fp32)
 Tensor linear_xent_bwd(Tensor gloss, Tensor xp, bool x_f32, Tensor w, c10::optional<Tensor> b, Tensor target,
                        int64_t ignore, bool bf16_products, Tensor lse, Tensor inv_count, bool want_dx,
-                       c10::optional<Tensor> dw, c10::optional<Tensor> db, bool accumulate) {
+                       c10::optional<Tensor> dw, c10::optional<Tensor> db, bool accumulate, Tensor kept) {
   pmd::LxIo io{};
   const pmd::LxShape s = lx_shape(target.numel(), w.size(-1), x_f32, w, b, target, bf16_products, io);
   CHECK_F32(gloss); CHECK_F32(lse); CHECK_F32(inv_count); CHECK_CONT(lse); CHECK_CONT(xp);
   TORCH_CHECK(gloss.device() == w.device() && lse.device() == w.device() && inv_count.device() == w.device() &&
               xp.device() == w.device() && xp.scalar_type() == torch::kBFloat16 && xp.numel() == pmd::lx_xplanes(s) &&
-              gloss.numel() == 1 && inv_count.numel() == 1 && lse.numel() == s.N, "linear_xent: saved tensors");
+              gloss.numel() == 1 && inv_count.numel() == 1 && lse.numel() == s.N && kept.device() == w.device() &&
+              kept.scalar_type() == torch::kUInt8 && (kept.numel() == 0 || kept.numel() == pmd::lx_kept_bytes(s)),
+              "linear_xent: saved tensors");
   c10::DeviceGuard g(w.device());
   Tensor dx;
   if (want_dx) {
@@ -966,7 +973,8 @@ Tensor linear_xent_bwd(Tensor gloss, Tensor xp, bool x_f32, Tensor w, c10::optio
     }
     return dx;
   }
-  Tensor ws = torch::empty({pmd::lx_workspace_bytes(s, true)}, w.options().dtype(torch::kUInt8));
+  Tensor ws = torch::empty({pmd::lx_workspace_bytes(s, true, kept.numel() > 0)}, w.options().dtype(torch::kUInt8));
+  if (kept.numel()) io.kept = kept.data_ptr();
   io.ignore = ignore;
   io.ws = ws.data_ptr();
   io.xp = xp.data_ptr();
@@ -992,6 +1000,14 @@ static variable_list once(variable_list g, const char* what) {
   auto err = std::make_shared<torch::autograd::DelayedError>(
       std::string("trying to differentiate twice through ") + what, (int)g.size());
   return (*err)(std::move(g));
+}
+
+// a call without gradients keeps nothing for a backward
+static bool wants_grad(std::initializer_list<const Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const Tensor* t : ts)
+    if (t && t->defined() && t->requires_grad()) return true;
+  return false;
 }
 
 struct GroupNormActNode : torch::autograd::Function<GroupNormActNode> {
@@ -1026,8 +1042,7 @@ struct GroupNormActNode : torch::autograd::Function<GroupNormActNode> {
 };
 Tensor group_norm_act(Tensor x, Tensor weight, Tensor bias, c10::optional<Tensor> res, int64_t groups, double eps,
                       int64_t act) {
-  const bool r = res && res->defined() && res->requires_grad();
-  if (!at::GradMode::is_enabled() || !(x.requires_grad() || weight.requires_grad() || bias.requires_grad() || r))
+  if (!wants_grad({&x, &weight, &bias, res ? &*res : nullptr}))
     return group_norm_fwd(x, res, weight, bias, groups, eps, act, false)[0];
   return GroupNormActNode::apply(x, weight, bias, res, groups, eps, act);
 }
@@ -1035,9 +1050,9 @@ Tensor group_norm_act(Tensor x, Tensor weight, Tensor bias, c10::optional<Tensor
 struct LinearXentNode : torch::autograd::Function<LinearXentNode> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const c10::optional<Tensor>& b,
                                const Tensor& target, int64_t ignore, bool bf16) {
-    auto r = linear_xent_fwd(x, w, b, target, ignore, bf16);
     const bool bias = b && b->defined();
-    ctx->save_for_backward({r[4], w, bias ? *b : Tensor(), target, r[2], r[3]});
+    auto r = linear_xent_fwd(x, w, b, target, ignore, bf16, true);
+    ctx->save_for_backward({r[4], w, bias ? *b : Tensor(), target, r[2], r[3], r[5]});
     ctx->saved_data["ignore"] = ignore;
     ctx->saved_data["bf16"] = bf16;
     ctx->saved_data["x_f32"] = x.scalar_type() == torch::kFloat32;
@@ -1060,7 +1075,7 @@ struct LinearXentNode : torch::autograd::Function<LinearXentNode> {
       if (ctx->saved_data["db"].toBool()) db = torch::empty_like(s[2]);
       out[0] = linear_xent_bwd(g[0].reshape({1}), s[0], ctx->saved_data["x_f32"].toBool(), s[1], s[2], s[3],
                                ctx->saved_data["ignore"].toInt(), ctx->saved_data["bf16"].toBool(), s[4], s[5],
-                               ctx->saved_data["dx"].toBool(), dw, db, false);
+                               ctx->saved_data["dx"].toBool(), dw, db, false, s[6]);
       out[1] = dw;
       out[2] = db;
     }
@@ -1068,6 +1083,10 @@ struct LinearXentNode : torch::autograd::Function<LinearXentNode> {
   }
 };
 std::vector<Tensor> linear_xent(Tensor x, Tensor w, c10::optional<Tensor> b, Tensor target, int64_t ignore, bool bf16) {
+  if (!wants_grad({&x, &w, b ? &*b : nullptr})) {
+    auto r = linear_xent_fwd(x, w, b, target, ignore, bf16, false);
+    return {r[0].reshape({}), r[1]};
+  }
   return LinearXentNode::apply(x, w, b, target, ignore, bf16);
 }
 

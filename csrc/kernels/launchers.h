@@ -208,6 +208,7 @@ struct LxIo {
   void* ws;                          // lx_workspace_bytes
   void* xp;                          // lx_xplanes bf16: x laid out, rows to ignore zero; the forward's output,
                                      // the backward's input (which needs no x)
+  void* kept;                        // nullable: lx_kept_bytes, the forward's output and its backward's input
   float *loss, *lse, *inv_count;     // [1], [N], [1]; lse and inv_count are the backward's inputs
   long long* correct;                // [1]
   const float* gloss;                // backward: d(loss) [1]
@@ -215,7 +216,8 @@ struct LxIo {
   bool dw_f32, accumulate;           // accumulate: dw, db (fp32) +=
 };
 long long lx_xplanes(const LxShape& s);
-long long lx_workspace_bytes(const LxShape& s, bool bwd);
+long long lx_workspace_bytes(const LxShape& s, bool bwd, bool kept);
+long long lx_kept_bytes(const LxShape& s);  // 0: too much to keep
 int lx_fwd_launch(const LxShape& s, const LxIo& io, hipStream_t st);
 int lx_bwd_launch(const LxShape& s, const LxIo& io, hipStream_t st);
 

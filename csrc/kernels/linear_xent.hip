@@ -6,14 +6,18 @@
 //
 // The logits are never stored.  Forward: the product's epilogue reduces its tile to (max, sum of
 // exponentials, argmax) per row, one combine pass joins the column tiles, one block sums the rows.
-// Backward, per piece of the vocabulary: the piece's logits are computed again and their epilogue
-// writes softmax - onehot in 16 bits (a piece holds at most kPieceBytes, which the last-level cache
-// keeps); the two gradient products read it from there.  That is 8 N V D operations where keeping
-// the logits would need 6.
+// When a backward will follow, the epilogue also keeps the exponentials it has at hand, about the
+// maximum of their row in the wave's columns, if they take at most kKeepBytes.
+// Backward, per piece of the vocabulary: softmax - onehot is written in 16 bits (a piece holds at most
+// kPieceBytes, which the last-level cache keeps) and the two gradient products read it from there.  It
+// comes from the kept exponentials, times exp(their maximum - lse), in a pass bound by memory; or, past
+// kKeepBytes, from the piece's logits computed again, 8 N V D operations instead of 6.
 //
 // Rounding: operands are bf16 (products are then exact in fp32), or fp32 held as three bf16 planes
 // (gemm_core.h).  softmax - onehot is rounded to the same: one bf16 when the operands are bf16 --
 // half a bf16 step of each probability, the size of the gradients' own rounding -- or three planes.
+// Exponentials are kept in fp32 for fp32 operands, else in fp16 times 2^15: half an fp16 step (an
+// eighth of a bf16 one) down to 2^-29 of the maximum, and below that 2^-40 of it.
 // Sums, statistics, the loss and db stay in fp32 (db sums the probabilities before that rounding).
 // No atomics: partial results are joined in a fixed order.
 //
@@ -26,6 +30,8 @@ namespace pmd {
 namespace {
 
 constexpr long long kPieceBytes = 192ll << 20;
+constexpr long long kKeepBytes = 4ll << 30;
+constexpr float kKeepScale = 32768.f;  // exponentials of at most 1 as fp16: up to 2^15 (its largest is 65504)
 
 __device__ __forceinline__ float ld_any(const void* p, long long i, bool f32) {
   return f32 ? static_cast<const float*>(p)[i] : bf2f(static_cast<const bf16_t*>(p)[i]);
@@ -79,6 +85,9 @@ struct LxArgs {
   float *pmax, *psum;    // [column tiles][N]
   int* pidx;
   float* tlogit;         // [N]
+  void* keep;            // nullable: exponentials [N][ldk], fp32 or (one plane) fp16 times kKeepScale
+  float* kref;           // [V / the waves' columns][N]: what they are about
+  long long ldk;
   // backward
   const float* lse;      // [N]
   bf16_t* prob;          // PL planes [N][ldp]
@@ -89,6 +98,41 @@ struct LxArgs {
 
 __device__ __forceinline__ float bias_of(const void* bias, int f32, int n, int V) {
   return bias && n < V ? ld_any(bias, n, f32) : 0.f;
+}
+
+typedef float f32x4_keep __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x4_keep __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8_keep __attribute__((ext_vector_type(8)));
+
+// read once, in the backward: the stores and loads leave the caches to the operands
+template <int PL>
+__device__ __forceinline__ void keep_store(void* p, long long o, const float (&v)[4]) {
+  if constexpr (PL == 1) {
+    f16x4_keep h;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) h[e] = (_Float16)(v[e] * kKeepScale);
+    __builtin_nontemporal_store(h, reinterpret_cast<f16x4_keep*>(static_cast<_Float16*>(p) + o));
+  } else {
+    const f32x4_keep h = {v[0], v[1], v[2], v[3]};
+    __builtin_nontemporal_store(h, reinterpret_cast<f32x4_keep*>(static_cast<float*>(p) + o));
+  }
+}
+template <int PL>
+__device__ __forceinline__ void keep_load(const void* p, long long o, float (&v)[8]) {
+  if constexpr (PL == 1) {
+    const f16x8_keep h =
+        __builtin_nontemporal_load(reinterpret_cast<const f16x8_keep*>(static_cast<const _Float16*>(p) + o));
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = (float)h[e];
+  } else {
+    const f32x4_keep* q = reinterpret_cast<const f32x4_keep*>(static_cast<const float*>(p) + o);
+    const f32x4_keep h0 = __builtin_nontemporal_load(q), h1 = __builtin_nontemporal_load(q + 1);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      v[e] = h0[e];
+      v[4 + e] = h1[e];
+    }
+  }
 }
 
 // ---------------------------------------------------------------- forward
@@ -149,9 +193,16 @@ __global__ __launch_bounds__(G::NT) void lx_fwd_kernel(LxArgs<G::PL> a) {
     const float ref = mx == -INFINITY ? 0.f : mx;  // nothing above -inf: the sum is 0, not NaN
     float s = 0.f;
 #pragma unroll
-    for (int j = 0; j < G::NI; ++j)
+    for (int j = 0; j < G::NI; ++j) {
+      float v[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s += __expf(acc[i][j][e] - ref);
+      for (int e = 0; e < 4; ++e) {
+        v[e] = __expf(acc[i][j][e] - ref);
+        s += v[e];
+      }
+      if (a.keep && m < a.N && nb + j * 16 < a.ldk) keep_store<G::PL>(a.keep, m * a.ldk + nb + j * 16, v);
+    }
+    if (a.keep && lane < 16 && m < a.N) a.kref[(long long)(in * G::WN + wn) * a.N + m] = mx;
     s += __shfl_xor(s, 16, 64);
     s += __shfl_xor(s, 32, 64);
     if (lane < 16) {
@@ -375,6 +426,74 @@ __global__ __launch_bounds__(G::NT) void lx_prob_kernel(LxArgs<G::PL> a) {
   }
 }
 
+// The same from the exponentials that the forward kept, in blocks of `rows` rows x CW vectors of 8 columns;
+// the 256 / CW groups of threads take consecutive rows each.  8,192 rows x 8,192 columns in KEEPTIME us
+// (KEEPBW TB/s read and written); computing the logits again takes 265 us.
+template <int PL>
+struct LxScale {
+  const void* keep;       // from the piece's first class
+  const float *kref, *lse, *tlogit;
+  long long ldk;
+  int kshift;             // log2 of the columns that share a kref
+  const long long* target;
+  long long ignore;
+  int N, V, v0;           // V: classes of the piece
+  bf16_t* prob;
+  long long pplane;
+  int ldp, CW, rows, cblocks;
+  float* dbpart;
+};
+template <int PL>
+__global__ __launch_bounds__(256) void lx_scale_kernel(LxScale<PL> a) {
+  __shared__ float sc[256 * 9];
+  const int tid = threadIdx.x, tc = tid & (a.CW - 1), grp = tid / a.CW, per = a.rows * a.CW / 256;
+  const int im = blockIdx.x / a.cblocks, cb = blockIdx.x - im * a.cblocks;
+  const int n = (cb * a.CW + tc) * 8, ms = im * a.rows + grp * per, me = min(a.N, ms + per);
+  float col[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) col[e] = 0.f;
+  if (n < a.ldp) {
+    const float* ref = a.kref + (long long)((a.v0 + n) >> a.kshift) * a.N;
+#pragma unroll 4
+    for (int m = ms; m < me; ++m) {
+      float v[8];
+      keep_load<PL>(a.keep, m * a.ldk + n, v);
+      const long long t = a.target[m];
+      const bool keep = t != a.ignore;
+      const float lse = a.lse[m];
+      const float s = __expf(ref[m] - lse) * (PL == 1 ? 1.f / kKeepScale : 1.f);
+      const long long d = t - a.v0 - n;  // the target among the 8
+      bf16_t o[8][PL];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float p = 0.f;
+        if (keep && n + e < a.V) p = d == e ? __expf(a.tlogit[m] - lse) - 1.f : v[e] * s;
+        col[e] += p;
+        to_planes<PL>(p, o[e]);
+      }
+#pragma unroll
+      for (int q = 0; q < PL; ++q) {
+        uint32_t w[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[k] = (uint32_t)o[2 * k][q] | ((uint32_t)o[2 * k + 1][q] << 16);
+        *reinterpret_cast<uint4*>(a.prob + q * a.pplane + (long long)m * a.ldp + n) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+  }
+  if (!a.dbpart) return;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) sc[tid * 9 + e] = col[e];
+  __syncthreads();
+  if (grp == 0 && n < a.ldp) {
+    for (int g = 1; g < 256 / a.CW; ++g)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) col[e] += sc[(g * a.CW + tc) * 9 + e];
+    float* d = a.dbpart + (long long)im * a.ldp + n;
+    *reinterpret_cast<float4*>(d) = make_float4(col[0], col[1], col[2], col[3]);
+    *reinterpret_cast<float4*>(d + 4) = make_float4(col[4], col[5], col[6], col[7]);
+  }
+}
+
 __device__ __forceinline__ void st4(void* p, bool f32, long long o, const float (&v)[4], int n, bool acc) {
   if (f32) {
     float* d = static_cast<float*>(p) + o;
@@ -568,7 +687,11 @@ struct LxPlan {
   bool w_direct;            // the weight is read in place
   int fwd_tile, fwd_ct;     // forward tile and column tiles
   int piece, pieces;        // classes of a piece (multiple of 64 unless it is all of V), pieces
-  int bwd_tile, bwd_rt;     // tile and row tiles of the recomputation
+  int kshift;               // log2 of the forward's columns of a wave
+  long long ldk;            // row of the kept exponentials
+  bool keep;                // they are within kKeepBytes
+  int bwd_tile, bwd_rt;     // tile of the recomputation; its row tiles, or those of lx_scale_kernel
+  int sc_cw, sc_rows;       // lx_scale_kernel's column vectors and rows of a block
   int dx_tile, dx_splits, dx_ksplit, dw_tile;
 };
 
@@ -580,6 +703,14 @@ void lx_plan_piece(const LxShape& s, long long piece, LxPlan& p) {
   p.pieces = (s.V + p.piece - 1) / p.piece;
   p.bwd_tile = pick_tile(s.N, p.piece, 1, s.planes);
   p.bwd_rt = (s.N + p.bwd_tile - 1) / p.bwd_tile;
+  if (p.keep) {  // at least 4 rows a thread, and four blocks a compute unit where that leaves them
+    const int vecs = up(p.piece, 64) / 8;
+    for (p.sc_cw = 8; p.sc_cw < 64 && p.sc_cw * 2 <= vecs;) p.sc_cw *= 2;
+    const long long cb = (vecs + p.sc_cw - 1) / p.sc_cw;
+    for (p.sc_rows = 128; p.sc_rows > 4 * 256 / p.sc_cw && cb * ((s.N + p.sc_rows - 1) / p.sc_rows) < 1024;)
+      p.sc_rows /= 2;
+    p.bwd_rt = (s.N + p.sc_rows - 1) / p.sc_rows;
+  }
   p.dw_tile = pick_tile(p.piece, p.Dp, 1, s.planes);
   // dx reduces over the classes: split them until the compute units are full, at least 512 a split
   p.dx_tile = pick_tile(s.N, p.Dp, (int)(p.piece / 512 > 0 ? p.piece / 512 : 1), s.planes);
@@ -601,12 +732,16 @@ long long lx_piece_cost(const LxShape& s, const LxPlan& p) {
   return p.pieces * (prob + dw + dx);
 }
 
-LxPlan lx_plan(const LxShape& s) {
+// kept: the exponentials are kept if they are few enough
+LxPlan lx_plan(const LxShape& s, bool kept) {
   LxPlan p;
   p.Dp = up(s.D, 8);
   p.w_direct = s.planes == 1 && !s.w_f32 && s.D % 8 == 0 && s.w_aligned;
   p.fwd_tile = pick_tile(s.N, s.V, 1, s.planes);
   p.fwd_ct = (s.V + p.fwd_tile - 1) / p.fwd_tile;
+  p.kshift = p.fwd_tile == 64 ? 5 : 6;
+  p.ldk = up(s.V, 64);
+  p.keep = kept && s.N * (p.ldk + (p.ldk >> p.kshift) * 2) * (s.planes == 1 ? 2 : 4) <= kKeepBytes;
   const int vp = up(s.V, 64);
   long long piece = kPieceBytes / (2ll * s.planes * s.N) / 256 * 256;
   if (piece < 1024) piece = 1024;
@@ -670,6 +805,20 @@ LxBuf lx_carve(const LxShape& s, const LxPlan& p, bool bwd, char* base, long lon
   return b;
 }
 
+struct LxKept {  // what a forward keeps for its backward
+  void* e;
+  float *ref, *tlogit;
+};
+LxKept lx_kept(const LxShape& s, const LxPlan& p, void* base, long long* bytes) {
+  Carver c{static_cast<char*>(base)};
+  LxKept k{};
+  k.e = c.take<char>(s.N * p.ldk * (s.planes == 1 ? 2 : 4));
+  k.ref = c.take<float>((long long)s.N * (up(s.V, p.fwd_tile) >> p.kshift));
+  k.tlogit = c.take<float>(s.N);
+  *bytes = c.off;
+  return k;
+}
+
 template <int PL>
 GemmOperand<PL> planes_of(const bf16_t* p, long long plane, long long ld, int rows) {
   GemmOperand<PL> o;
@@ -694,9 +843,11 @@ bool lx_ok(const LxShape& s) {
 
 template <int PL>
 int lx_fwd_t(const LxShape& s, const LxIo& io, hipStream_t st) {
-  const LxPlan p = lx_plan(s);
+  const LxPlan p = lx_plan(s, io.kept != nullptr);
   long long bytes;
   LxBuf b = lx_carve(s, p, false, static_cast<char*>(io.ws), &bytes);
+  const LxKept kept = lx_kept(s, p, io.kept, &bytes);
+  if (io.kept) b.tlogit = kept.tlogit;
   b.x = static_cast<bf16_t*>(io.xp);
   lx_prep<PL>(io.x, s.x_f32, s.N, s.D, b.x, p.Dp, io.target, io.ignore, st);
   if (!p.w_direct) lx_prep<PL>(io.w, s.w_f32, s.V, s.D, b.w, p.Dp, nullptr, 0, st);
@@ -708,6 +859,7 @@ int lx_fwd_t(const LxShape& s, const LxIo& io, hipStream_t st) {
   a.bias = io.bias; a.bias_f32 = s.b_f32;
   a.target = io.target; a.ignore = io.ignore;
   a.pmax = b.pmax; a.psum = b.psum; a.pidx = b.pidx; a.tlogit = b.tlogit;
+  a.keep = kept.e; a.kref = kept.ref; a.ldk = p.ldk;
   const int rc = with_tile<PL, false, false>(p.fwd_tile, [&](auto g) {
     using G = decltype(g);
     hipLaunchKernelGGL(lx_fwd_kernel<G>, dim3((unsigned)tiles_of(s.N, s.V, G::BM)), dim3(G::NT), 0, st, a);
@@ -727,11 +879,12 @@ int lx_fwd_t(const LxShape& s, const LxIo& io, hipStream_t st) {
 
 template <int PL>
 int lx_bwd_t(const LxShape& s, const LxIo& io, hipStream_t st) {
-  const LxPlan p = lx_plan(s);
+  const LxPlan p = lx_plan(s, io.kept != nullptr);
   long long bytes;
   LxBuf b = lx_carve(s, p, true, static_cast<char*>(io.ws), &bytes);
   b.x = static_cast<bf16_t*>(io.xp);  // the forward's
-  if (!p.w_direct) lx_prep<PL>(io.w, s.w_f32, s.V, s.D, b.w, p.Dp, nullptr, 0, st);
+  const LxKept kept = lx_kept(s, p, io.kept, &bytes);
+  if (!p.w_direct && (!io.kept || io.dx)) lx_prep<PL>(io.w, s.w_f32, s.V, s.D, b.w, p.Dp, nullptr, 0, st);
   const bf16_t* wbase = p.w_direct ? static_cast<const bf16_t*>(io.w) : b.w;
   const long long wplane = p.w_direct ? 0 : (long long)s.V * p.Dp;
   for (int k = 0; k < p.pieces; ++k) {
@@ -747,7 +900,16 @@ int lx_bwd_t(const LxShape& s, const LxIo& io, hipStream_t st) {
     a.ldp = up(V, 64);
     a.prob = b.prob; a.pplane = (long long)s.N * a.ldp;
     a.dbpart = io.db ? b.dbpart : nullptr;
-    with_tile<PL, false, false>(p.bwd_tile, [&](auto g) {
+    if (io.kept) {
+      LxScale<PL> c{};
+      c.keep = static_cast<const char*>(kept.e) + (long long)v0 * (PL == 1 ? 2 : 4);
+      c.kref = kept.ref; c.lse = io.lse; c.tlogit = kept.tlogit;
+      c.ldk = p.ldk; c.kshift = p.kshift; c.target = io.target; c.ignore = io.ignore;
+      c.N = s.N; c.V = V; c.v0 = v0;
+      c.prob = b.prob; c.pplane = a.pplane; c.ldp = a.ldp; c.dbpart = a.dbpart;
+      c.CW = p.sc_cw; c.rows = p.sc_rows; c.cblocks = (a.ldp / 8 + c.CW - 1) / c.CW;
+      hipLaunchKernelGGL(lx_scale_kernel<PL>, dim3((unsigned)(c.cblocks * p.bwd_rt)), dim3(256), 0, st, c);
+    } else with_tile<PL, false, false>(p.bwd_tile, [&](auto g) {
       using G = decltype(g);
       hipLaunchKernelGGL(lx_prob_kernel<G>, dim3((unsigned)tiles_of(s.N, a.ldp, G::BM)), dim3(G::NT), 0, st, a);
       return 0;
@@ -808,10 +970,18 @@ int lx_bwd_t(const LxShape& s, const LxIo& io, hipStream_t st) {
 
 long long lx_xplanes(const LxShape& s) { return (long long)s.planes * s.N * up(s.D, 8); }
 
-long long lx_workspace_bytes(const LxShape& s, bool bwd) {
+long long lx_workspace_bytes(const LxShape& s, bool bwd, bool kept) {
   if (!lx_ok(s)) return 0;
   long long bytes;
-  lx_carve(s, lx_plan(s), bwd, nullptr, &bytes);
+  lx_carve(s, lx_plan(s, kept), bwd, nullptr, &bytes);
+  return bytes;
+}
+
+long long lx_kept_bytes(const LxShape& s) {
+  if (!lx_ok(s)) return 0;
+  const LxPlan p = lx_plan(s, true);
+  long long bytes = 0;
+  if (p.keep) lx_kept(s, p, nullptr, &bytes);
   return bytes;
 }
 

@@ -1591,6 +1591,8 @@ def group_norm_act(x, gn, residual=None, act="relu"):
     args = (x.contiguous(), gn.weight, gn.bias, residual, int(gn.num_groups), float(gn.eps), act)
     if _native_node(x, gn.weight, gn.bias):
         return prims_for(x).group_norm_act(*args)
+    if not torch.is_grad_enabled():
+        return prims_for(x).group_norm_fwd(args[0], residual, *args[1:3], *args[4:], False)[0]
     return _GroupNormActFn.apply(*args)
 
 
@@ -1694,14 +1696,16 @@ def cross_entropy(logits, target):
 
 
 class _LinearXentFn(torch.autograd.Function):
-    """(loss, correct) of a linear classifier without its logits; saves the operands and one
-    log-sum-exp per row, and computes the logits again, piece by piece, in the backward."""
+    """(loss, correct) of a linear classifier; saves the operands, one log-sum-exp per row, and the
+    exponentials in the operands' width unless they are too many, when the backward computes the logits
+    again, piece by piece."""
 
     @staticmethod
     def forward(ctx, x, w, b, target, ignore, bf16):
         P = prims_for(x)
-        loss, correct, lse, inv, xp = P.linear_xent_fwd(x, w, b, target, ignore, bf16)
-        ctx.save_for_backward(xp, w, b, target, lse, inv)
+        loss, correct, lse, inv, xp, kept = P.linear_xent_fwd(x, w, b, target, ignore, bf16,
+                                                              any(ctx.needs_input_grad))
+        ctx.save_for_backward(xp, w, b, target, lse, inv, kept)
         ctx.params = (w, b)
         ctx.cfg = (ignore, bf16, x.dtype)
         ctx.mark_non_differentiable(correct)
@@ -1713,7 +1717,7 @@ class _LinearXentFn(torch.autograd.Function):
     def backward(ctx, gloss, _gcorrect):
         if gloss is None:
             return (None,) * 6
-        xp, w, b, target, lse, inv = ctx.saved_tensors
+        xp, w, b, target, lse, inv, kept = ctx.saved_tensors
         wp, bp = ctx.params
         ignore, bf16, x_dtype = ctx.cfg
         P = prims_for(w)
@@ -1730,7 +1734,7 @@ class _LinearXentFn(torch.autograd.Function):
                 db = torch.empty_like(b)
         g = gloss.reshape(1).to(lse.dtype)
         dx = P.linear_xent_bwd(g, xp, x_dtype, w, b, target, ignore, bf16, lse, inv, ctx.needs_input_grad[0], dw, db,
-                               arena)
+                               arena, kept)
         if arena:
             _ready(wp, *([bp] if bp is not None else []))
             dw = db = None
@@ -1740,8 +1744,10 @@ class _LinearXentFn(torch.autograd.Function):
 def linear_cross_entropy(x, lin, target, ignore_index=-100, compute_dtype=None):
     """``(loss, correct)`` of the classifier ``lin`` on features ``x``: the mean softmax cross-entropy of
     ``x lin.weight^T + lin.bias`` and the top-1 count (int64 [1], on the device) -- what
-    :func:`linear`, :func:`cross_entropy` and :func:`correct_count` give, without keeping the [N, V]
-    logits: for classifiers of many classes.
+    :func:`linear`, :func:`cross_entropy` and :func:`correct_count` give, without the [N, V] logits and
+    their fp32 copies.  On a GPU a call with gradients keeps N x V exponentials in the products' width, up to
+    4 GiB; past that it keeps none, and the backward computes the logits again, a piece of the classes at a
+    time.
 
     ``x`` [..., D] and ``target`` [...] (int64 class indices); rows whose target is ``ignore_index`` count
     for nothing, whatever they hold, and get a zero gradient; when no row is left the loss is 0.  A
@@ -1765,6 +1771,9 @@ def linear_cross_entropy(x, lin, target, ignore_index=-100, compute_dtype=None):
             int(ignore_index), compute_dtype is not None)
     if _native_node(x, w, b):
         return prims_for(x).linear_xent(*args)
+    if not torch.is_grad_enabled():
+        loss, correct = prims_for(x).linear_xent_fwd(*args, False)[:2]
+        return loss.reshape(()), correct
     return _LinearXentFn.apply(*args)
 
 

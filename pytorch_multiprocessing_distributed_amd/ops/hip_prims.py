@@ -294,17 +294,18 @@ def xent_bwd(gloss, logits, target, lse):
     return g.to(logits.dtype)
 
 
-def linear_xent_fwd(x, w, b, target, ignore, bf16):
-    """-> (loss [1], correct [1], and for the backward: lse [N], 1 / kept rows [1], x laid out); no logits
-    are stored."""
+def linear_xent_fwd(x, w, b, target, ignore, bf16, want_grad):
+    """-> (loss [1], correct [1], and for the backward: lse [N], 1 / kept rows [1], x laid out, the
+    exponentials -- empty unless ``want_grad``, or if they are too many to keep)."""
     return tuple(_C.linear_xent_fwd(x, w.detach(), None if b is None else b.detach(), target, int(ignore),
-                                    bool(bf16)))
+                                    bool(bf16), bool(want_grad)))
 
 
-def linear_xent_bwd(gloss, xp, x_dtype, w, b, target, ignore, bf16, lse, inv_count, want_dx, dw, db, accumulate):
+def linear_xent_bwd(gloss, xp, x_dtype, w, b, target, ignore, bf16, lse, inv_count, want_dx, dw, db, accumulate, kept):
     """-> dx or None; ``dw`` / ``db`` (None: not wanted) are written, or added to (fp32 targets)."""
     return _C.linear_xent_bwd(gloss, xp, x_dtype == torch.float32, w.detach(), None if b is None else b.detach(),
-                              target, int(ignore), bool(bf16), lse, inv_count, bool(want_dx), dw, db, bool(accumulate))
+                              target, int(ignore), bool(bf16), lse, inv_count, bool(want_dx), dw, db, bool(accumulate),
+                              kept)
 
 
 def group_norm_act(x, weight, bias, res, groups, eps, act):

@@ -392,9 +392,9 @@ def _lx_operands(x, w, b, bf16):
     return op(x), op(w), None if b is None else _f(b.detach())
 
 
-def linear_xent_fwd(x, w, b, target, ignore, bf16):
+def linear_xent_fwd(x, w, b, target, ignore, bf16, want_grad):
     """Mean softmax cross-entropy of ``x w^T + b`` over the rows whose target is not ``ignore``:
-    (loss [1], top-1 count [1], lse [N], 1 / kept rows [1], x).  No row kept: loss 0.  A target outside
+    (loss [1], top-1 count [1], lse [N], 1 / kept rows [1], x, None).  No row kept: loss 0.  A target outside
     the classes makes its row's loss NaN."""
     xf, wf, bf = _lx_operands(x, w, b, bf16)
     keep = target != ignore
@@ -409,10 +409,10 @@ def linear_xent_fwd(x, w, b, target, ignore, bf16):
     correct = torch.zeros(1, dtype=torch.int64, device=x.device)
     if x.shape[0]:
         correct = ((logits.argmax(1) == target) & keep).sum().reshape(1)
-    return rows.sum().reshape(1) * inv, correct, torch.where(keep & ~valid, nan, lse), inv, x
+    return rows.sum().reshape(1) * inv, correct, torch.where(keep & ~valid, nan, lse), inv, x, None
 
 
-def linear_xent_bwd(gloss, x, x_dtype, w, b, target, ignore, bf16, lse, inv_count, want_dx, dw, db, accumulate):
+def linear_xent_bwd(gloss, x, x_dtype, w, b, target, ignore, bf16, lse, inv_count, want_dx, dw, db, accumulate, kept):
     """-> dx or None; ``dw`` / ``db`` (None: not wanted) are written, or added to."""
     xf, wf, bf = _lx_operands(x, w, b, bf16)
     keep = target != ignore

@@ -66,7 +66,9 @@ def _check(x, lin, t, gloss=1.0, bf16=False, **kw):
     assert correct.item() == correct_r
     # p: exp of a logit off by 2 l_err and its own steps; bf16 products round softmax - onehot once
     two = bf16 or dt == torch.bfloat16
-    p_rel = 2 * l_err + 32 * U32 + (UB if two else 2.0 ** -22)
+    # and take exponentials that were kept in fp16, half a step each
+    kept = 2.0 ** -11 if two else 0.0
+    p_rel = 2 * l_err + 32 * U32 + kept + (UB if two else 2.0 ** -22)
     n = x.shape[0]
     # onehot - softmax near 1 cancels: an absolute 2 l_err of the softmax, relative to |p - 1|'s ab share
     out = UB if dt == torch.bfloat16 else 0.0
@@ -82,7 +84,7 @@ def _check(x, lin, t, gloss=1.0, bf16=False, **kw):
     assert ((got[1].double() - dw_r).abs() <= wout * dw_r.abs() + (p_rel + sum_rel) * aw + extra * g * xmax * same).all()
     if lin.bias is not None:
         bout = UB if lin.bias.dtype == torch.bfloat16 else 0.0
-        assert ((got[2].double() - db_r).abs() <= bout * db_r.abs() + (2 * l_err + 32 * U32 + sum_rel) * ab
+        assert ((got[2].double() - db_r).abs() <= bout * db_r.abs() + (2 * l_err + 32 * U32 + kept + sum_rel) * ab
                 + extra * g * same).all()
     assert not got[0][t == -100].any()
     return loss, got
@@ -129,6 +131,37 @@ def test_vocabulary_in_pieces(monkeypatch):
     # 2^24 rows never fit a test; 98,304 rows leave a piece of 1,024 classes: three pieces, the last ragged
     x, lin, t = _case(98304, 16, 2100, torch.bfloat16, seed=6)
     _check(x, lin, t)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n,d,v", [(1, 8, 2), (65, 72, 129), (300, 40, 20011), (2300, 264, 9001), (70000, 16, 2100)])
+def test_with_and_without_kept_exponentials(n, d, v, dtype):
+    """The backward that computes the logits again agrees with the one that has their exponentials."""
+    x, lin, t = _case(n, d, v, dtype, seed=19)
+    P = OF.prims_for(x)
+    args = (lin.weight.detach(), lin.bias.detach(), t, -100, False)
+    x = x.detach()
+    loss, _, lse, inv, xp, kept = P.linear_xent_fwd(x, *args, True)
+    loss2, _, lse2, _, _, none = P.linear_xent_fwd(x, *args, False)
+    assert none.numel() == 0 < kept.numel() and torch.equal(loss, loss2) and torch.equal(lse, lse2)
+    one = torch.ones(1, device="cuda")
+    r = []
+    for k in (kept, none):
+        dw, db = torch.empty_like(lin.weight), torch.empty_like(lin.bias)
+        dx = P.linear_xent_bwd(one, xp, dtype, *args, lse, inv, True, dw, db, False, k)
+        r.append((dx.double(), dw.double(), db.double()))
+    _, _, _, _, _, ax, aw, ab, mag = _ref(x, lin.weight, lin.bias, t)
+    # what _check allows a side, twice: a logit's error in the exponential, the roundings of it, the sums;
+    # at the target, where the onehot cancels it, the absolute error of the exponential
+    e = 2 * (d / 4 + 40) * U32 * mag + 32 * U32
+    two = dtype == torch.bfloat16
+    rel = 2 * (e + (2.0 ** -11 + UB if two else 2.0 ** -22) + (max(n, v) / 4 + 64) * U32)
+    out = 2 * UB if two else 0.0
+    g = 1.0 / max(1, int((t != -100).sum()))
+    same = int(torch.bincount(t[t != -100]).max())
+    wmax, xmax = lin.weight.double().abs().max(), x.double().masked_fill((t == -100)[:, None], 0).abs().max()
+    for a, b, m, f in zip(r[0], r[1], (ax, aw, ab), (wmax, xmax * same, same)):
+        assert ((a - b).abs() <= out * b.abs() + rel * m + 2 * e * g * f).all()
 
 
 def test_unaligned_weight_and_features():
