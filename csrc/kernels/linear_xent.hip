@@ -101,22 +101,33 @@ __device__ __forceinline__ float bias_of(const void* bias, int f32, int n, int V
 }
 
 typedef float f32x4_keep __attribute__((ext_vector_type(4)));
-typedef _Float16 f16x4_keep __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8_keep __attribute__((ext_vector_type(8)));
 
-// read once, in the backward: the stores and loads leave the caches to the operands
-template <int PL>
-__device__ __forceinline__ void keep_store(void* p, long long o, const float (&v)[4]) {
-  if constexpr (PL == 1) {
-    f16x4_keep h;
+// Exponentials are kept in the order in which lanes hold them: of 32 columns, column 16 j + 4 q + e at
+// 8 q + 4 j + e, so that a lane (row, q) stores 16 bytes and four of them 64 bytes of a row.  (In column order,
+// 8 bytes a lane, the forward of 8,192 x 2,048 x 131,072 takes 4.9 ms; so it takes 4.2, keeping nothing 3.7;
+// nontemporal stores change nothing.)
+template <int PL, int NI>
+__device__ __forceinline__ void keep_store(void* p, long long o, const float (&v)[NI][4]) {
+  static_assert(NI % 2 == 0, "a wave's columns are multiples of 32");
 #pragma unroll
-    for (int e = 0; e < 4; ++e) h[e] = (_Float16)(v[e] * kKeepScale);
-    __builtin_nontemporal_store(h, reinterpret_cast<f16x4_keep*>(static_cast<_Float16*>(p) + o));
-  } else {
-    const f32x4_keep h = {v[0], v[1], v[2], v[3]};
-    __builtin_nontemporal_store(h, reinterpret_cast<f32x4_keep*>(static_cast<float*>(p) + o));
+  for (int j = 0; j < NI; j += 2) {
+    if constexpr (PL == 1) {
+      f16x8_keep h;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) h[e] = (_Float16)(v[j + e / 4][e % 4] * kKeepScale);
+      *reinterpret_cast<f16x8_keep*>(static_cast<_Float16*>(p) + o + j * 16) = h;
+    } else {
+      f32x4_keep* d = reinterpret_cast<f32x4_keep*>(static_cast<float*>(p) + o + j * 16);
+      const f32x4_keep h0 = {v[j][0], v[j][1], v[j][2], v[j][3]};
+      const f32x4_keep h1 = {v[j + 1][0], v[j + 1][1], v[j + 1][2], v[j + 1][3]};
+      d[0] = h0;
+      d[1] = h1;
+    }
   }
 }
+// the 8 values kept at o (a multiple of 8), of 4 + 4 columns; pairs of lanes then exchange four, so that each
+// has 8 columns in a row
 template <int PL>
 __device__ __forceinline__ void keep_load(const void* p, long long o, float (&v)[8]) {
   if constexpr (PL == 1) {
@@ -132,6 +143,15 @@ __device__ __forceinline__ void keep_load(const void* p, long long o, float (&v)
       v[e] = h0[e];
       v[4 + e] = h1[e];
     }
+  }
+}
+__device__ __forceinline__ int keep_column(int o) { return (o & ~31) + (o & 8) * 2 + ((o & 16) >> 1); }
+__device__ __forceinline__ void keep_exchange(float (&v)[8], bool odd) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float t = __shfl_xor(odd ? v[e] : v[4 + e], 1, 64);
+    if (odd) v[e] = t;
+    else v[4 + e] = t;
   }
 }
 
@@ -191,17 +211,17 @@ __global__ __launch_bounds__(G::NT) void lx_fwd_kernel(LxArgs<G::PL> a) {
       }
     }
     const float ref = mx == -INFINITY ? 0.f : mx;  // nothing above -inf: the sum is 0, not NaN
-    float s = 0.f;
+    float s = 0.f, v[G::NI][4];
 #pragma unroll
-    for (int j = 0; j < G::NI; ++j) {
-      float v[4];
+    for (int j = 0; j < G::NI; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        v[e] = __expf(acc[i][j][e] - ref);
-        s += v[e];
+        v[j][e] = __expf(acc[i][j][e] - ref);
+        s += v[j][e];
       }
-      if (a.keep && m < a.N && nb + j * 16 < a.ldk) keep_store<G::PL>(a.keep, m * a.ldk + nb + j * 16, v);
-    }
+    const int nw = n0 + wn * G::TN;
+    if (a.keep && m < a.N && nw < a.ldk)
+      keep_store<G::PL, G::NI>(a.keep, m * a.ldk + nw + (lane >> 4) * 8, v);
     if (a.keep && lane < 16 && m < a.N) a.kref[(long long)(in * G::WN + wn) * a.N + m] = mx;
     s += __shfl_xor(s, 16, 64);
     s += __shfl_xor(s, 32, 64);
@@ -243,15 +263,16 @@ struct LxRows {  // the forward's per-tile results and what joining them gives
   int* hit;            // [N] 0: to ignore, 1: kept, 2: kept and top-1 right
 };
 
-// Joins the column tiles of 16 rows m0..; thread (r, q) of 256 takes every 16th tile of row r.  All threads
-// of the block call this (`t`: the thread's number among its 256).
-__device__ __forceinline__ void lx_join_rows(const LxRows& a, int m0, int t, float (*sm)[17], float (*ss)[17],
-                                             int (*si)[17]) {
-  const int r = t & 15, q = t >> 4, m = m0 + r;
+// Joins the column tiles of RB rows m0..; thread (r, q) takes every Q-th tile of row r.  All RB Q threads of
+// the block call this.
+template <int RB, int Q>
+__device__ __forceinline__ void lx_join_rows(const LxRows& a, int m0, float (*sm)[RB + 1], float (*ss)[RB + 1],
+                                             int (*si)[RB + 1]) {
+  const int r = threadIdx.x % RB, q = threadIdx.x / RB, m = m0 + r;
   float mx = -INFINITY, s = 0.f;
   int mi = 0x7fffffff;
   if (m < a.N)
-    for (int c = q; c < a.tiles; c += 16) {
+    for (int c = q; c < a.tiles; c += Q) {
       const long long o = (long long)c * a.N + m;
       const float om = a.pmax[o], os = a.psum[o];
       const int oi = a.pidx[o];
@@ -268,14 +289,14 @@ __device__ __forceinline__ void lx_join_rows(const LxRows& a, int m0, int t, flo
   si[q][r] = mi;
   __syncthreads();
   if (q == 0 && m < a.N) {
-    for (int k = 1; k < 16; ++k)
+    for (int k = 1; k < Q; ++k)
       if (sm[k][r] > mx || (sm[k][r] == mx && si[k][r] < mi)) {
         mx = sm[k][r];
         mi = si[k][r];
       }
     const float ref = mx == -INFINITY ? 0.f : mx;
     s = 0.f;
-    for (int k = 0; k < 16; ++k) s += sm[k][r] == -INFINITY ? ss[k][r] : ss[k][r] * __expf(sm[k][r] - ref);
+    for (int k = 0; k < Q; ++k) s += sm[k][r] == -INFINITY ? ss[k][r] : ss[k][r] * __expf(sm[k][r] - ref);
     const long long t0 = a.target[m];
     const bool keep = t0 != a.ignore, in = t0 >= 0 && t0 < a.V;
     const float l = mx + __logf(s);
@@ -288,7 +309,7 @@ __device__ __forceinline__ void lx_join_rows(const LxRows& a, int m0, int t, flo
 __global__ __launch_bounds__(256) void lx_combine_kernel(LxRows a) {
   __shared__ float sm[16][17], ss[16][17];
   __shared__ int si[16][17];
-  lx_join_rows(a, blockIdx.x * 16, threadIdx.x, sm, ss, si);
+  lx_join_rows<16, 16>(a, blockIdx.x * 16, sm, ss, si);
 }
 
 // loss = sum of the row losses / kept, correct, 1 / kept
@@ -331,14 +352,14 @@ __global__ __launch_bounds__(1024) void lx_loss_kernel(const float* __restrict__
                                                        float* __restrict__ inv_count) {
   lx_total(rloss, hit, N, loss, correct, inv_count);
 }
-// both in one block, for few results: 64 rows at a time
-constexpr int kOneBlock = 16384;  // rows x tiles
+// both in one block, 256 rows at a time, for up to 512 rows and 64 tiles: 256 rows of 16 tiles take 5.7 us (1,030
+// rows of 65 tiles take lx_combine_kernel 10.4 and lx_loss_kernel 3.9)
+constexpr int kOneBlockRows = 512, kOneBlockTiles = 64;
 __global__ __launch_bounds__(1024) void lx_finish_kernel(LxRows a, float* loss, long long* correct, float* inv_count) {
-  __shared__ float sm[4][16][17], ss[4][16][17];
-  __shared__ int si[4][16][17];
-  const int part = threadIdx.x >> 8;
-  for (int m0 = 0; m0 < a.N; m0 += 64) {
-    lx_join_rows(a, m0 + part * 16, threadIdx.x & 255, sm[part], ss[part], si[part]);
+  __shared__ float sm[4][257], ss[4][257];
+  __shared__ int si[4][257];
+  for (int m0 = 0; m0 < a.N; m0 += 256) {
+    lx_join_rows<256, 4>(a, m0, sm, ss, si);
     __syncthreads();
   }
   __threadfence_block();
@@ -427,8 +448,8 @@ __global__ __launch_bounds__(G::NT) void lx_prob_kernel(LxArgs<G::PL> a) {
 }
 
 // The same from the exponentials that the forward kept, in blocks of `rows` rows x CW vectors of 8 columns;
-// the 256 / CW groups of threads take consecutive rows each.  8,192 rows x 8,192 columns in KEEPTIME us
-// (KEEPBW TB/s read and written); computing the logits again takes 265 us.
+// the 256 / CW groups of threads take consecutive rows each.  8,192 rows x 8,192 columns in 53 us (5.0 TB/s
+// read and written); computing the logits again takes 265 us.
 template <int PL>
 struct LxScale {
   const void* keep;       // from the piece's first class
@@ -448,7 +469,7 @@ __global__ __launch_bounds__(256) void lx_scale_kernel(LxScale<PL> a) {
   __shared__ float sc[256 * 9];
   const int tid = threadIdx.x, tc = tid & (a.CW - 1), grp = tid / a.CW, per = a.rows * a.CW / 256;
   const int im = blockIdx.x / a.cblocks, cb = blockIdx.x - im * a.cblocks;
-  const int n = (cb * a.CW + tc) * 8, ms = im * a.rows + grp * per, me = min(a.N, ms + per);
+  const int o8 = (cb * a.CW + tc) * 8, n = keep_column(o8), ms = im * a.rows + grp * per, me = min(a.N, ms + per);
   float col[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) col[e] = 0.f;
@@ -457,7 +478,8 @@ __global__ __launch_bounds__(256) void lx_scale_kernel(LxScale<PL> a) {
 #pragma unroll 4
     for (int m = ms; m < me; ++m) {
       float v[8];
-      keep_load<PL>(a.keep, m * a.ldk + n, v);
+      keep_load<PL>(a.keep, m * a.ldk + o8, v);
+      keep_exchange(v, tc & 1);
       const long long t = a.target[m];
       const bool keep = t != a.ignore;
       const float lse = a.lse[m];
@@ -585,7 +607,7 @@ __global__ __launch_bounds__(GX::NT) void lx_grads_kernel(LxGradArgs<GX::PL> x, 
   else lx_grad_tile<GW>(w, b - xblocks, wblocks, 0, smem);
 }
 
-// The last kernel of a piece: db [V] = or += scale * column sums of part [tiles][ldp], in blocks of 256
+// The last kernel of a piece: db [V] = or += scale * column sums of part [tiles][ldp], in blocks of 64
 // classes; and after the last piece dx [M][cols] = scale * sum over the slabs [splits][M][ld] (rows to
 // ignore are zero), in the blocks behind them.
 struct LxTail {
@@ -600,10 +622,17 @@ struct LxTail {
 __global__ __launch_bounds__(256) void lx_tail_kernel(LxTail a) {
   const float sc = a.gloss[0] * a.inv_count[0];
   if ((int)blockIdx.x < a.db_blocks) {
-    const int n = blockIdx.x * 256 + threadIdx.x;
-    if (n >= a.V) return;
+    __shared__ float part[4][64];
+    const int g = threadIdx.x >> 6, n = blockIdx.x * 64 + (threadIdx.x & 63);
     float s = 0.f;
-    for (int t = 0; t < a.tiles; ++t) s += a.part[(long long)t * a.ldp + n];
+    if (n < a.V) {
+#pragma unroll 8
+      for (int t = g; t < a.tiles; t += 4) s += a.part[(long long)t * a.ldp + n];
+    }
+    part[g][threadIdx.x & 63] = s;
+    __syncthreads();
+    if (g || n >= a.V) return;
+    for (int k = 1; k < 4; ++k) s += part[k][threadIdx.x];
     s *= sc;
     if (a.db_f32) {
       float* d = static_cast<float*>(a.db) + n;
@@ -749,7 +778,8 @@ LxPlan lx_plan(const LxShape& s, bool kept) {
   lx_plan_piece(s, piece < vp ? piece : vp, p);
   if (p.pieces > 1 && p.bwd_tile == 256 && p.dw_tile == 256 && p.dx_tile == 256) {
     // a smaller piece may fill the last rounds better: 8,192 rows x 2,048 features x 131,072 classes take
-    // 16 pieces of 8,192 (17.3 ms) rather than 11 of 12,288 (18.9 ms), whose dw products have 384 blocks
+    // 16 pieces of 8,192 rather than 11 of 12,288, whose dW products have 384 blocks (18.9 ms, when the pieces of
+    // 8,192 took 16.6)
     long long best = lx_piece_cost(s, p), at = p.piece;
     for (long long c = piece - 256; c >= piece / 4; c -= 256) {
       lx_plan_piece(s, c, p);
@@ -867,7 +897,7 @@ int lx_fwd_t(const LxShape& s, const LxIo& io, hipStream_t st) {
   });
   if (rc) return rc;
   const LxRows r{b.pmax, b.psum, b.tlogit, b.pidx, io.target, io.ignore, s.N, s.V, p.fwd_ct, io.lse, b.rloss, b.hit};
-  if ((long long)s.N * p.fwd_ct <= kOneBlock) {
+  if (s.N <= kOneBlockRows && p.fwd_ct <= kOneBlockTiles) {
     hipLaunchKernelGGL(lx_finish_kernel, dim3(1), dim3(1024), 0, st, r, io.loss, io.correct, io.inv_count);
   } else {
     hipLaunchKernelGGL(lx_combine_kernel, dim3((s.N + 15) / 16), dim3(256), 0, st, r);
@@ -953,7 +983,7 @@ int lx_bwd_t(const LxShape& s, const LxIo& io, hipStream_t st) {
       if (io.db) {
         t.part = b.dbpart; t.tiles = p.bwd_rt; t.ldp = a.ldp; t.V = V;
         t.db = static_cast<char*>(io.db) + (long long)v0 * bsz; t.db_f32 = s.b_f32; t.accumulate = io.accumulate;
-        t.db_blocks = (V + 255) / 256;
+        t.db_blocks = (V + 63) / 64;
       }
       long long nb = 0;
       if (last && io.dx) {
