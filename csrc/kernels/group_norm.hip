@@ -7,6 +7,9 @@
 //     dx = rstd (gamma dz - mean(gamma dz) - xhat mean(gamma dz xhat))
 //     dgamma = sum_{n,hw} dz xhat,  dbeta = sum_{n,hw} dz
 //
+// These kernels read the data twice; samples whose groups fit a block's registers are taken by
+// kernels/group_norm_one.hip, which reads them once.
+//
 // Every pass is bound by memory; a thread owns VEC consecutive channels (16 bytes where the
 // channel count and the pointers allow) and walks down the pixels, so any group width works
 // the same way: statistics are taken per channel and joined into groups through LDS.
@@ -22,7 +25,7 @@
 // first four, and such triples are joined pairwise (Chan, Golub, LeVeque 1983).  Plain sums of x and x^2
 // would lose (mu/sigma)^2 of their precision; this loses at most kSeg 2^-24, when one of the four is far
 // off.  All joins run in a fixed order: results do not depend on the scheduling.
-#include "common.h"
+#include "group_norm.h"
 
 #include <algorithm>
 #include <initializer_list>
@@ -36,55 +39,6 @@ constexpr int GT = 256;   // threads of a block
 constexpr int GU = 4;    // pixels a thread loads at once
 constexpr int kSeg = 64;  // pixels a thread sums about one shift
 
-template <typename T>
-struct GnIo;
-template <>
-struct GnIo<bf16_t> {
-  static __device__ __forceinline__ float up(bf16_t v) { return bf2f(v); }
-  static __device__ __forceinline__ bf16_t down(float v) { return f2bf(v); }
-};
-template <>
-struct GnIo<float> {
-  static __device__ __forceinline__ float up(float v) { return v; }
-  static __device__ __forceinline__ float down(float v) { return v; }
-};
-
-template <typename T, int VEC>
-struct alignas(sizeof(T) * VEC) GnVec {
-  T v[VEC];
-};
-
-template <typename T, int VEC>
-__device__ __forceinline__ void gn_load(const T* p, float (&f)[VEC]) {
-  const GnVec<T, VEC> r = *reinterpret_cast<const GnVec<T, VEC>*>(p);
-#pragma unroll
-  for (int k = 0; k < VEC; ++k) f[k] = GnIo<T>::up(r.v[k]);
-}
-template <typename T, int VEC>
-__device__ __forceinline__ void gn_store(T* p, const float (&f)[VEC]) {
-  GnVec<T, VEC> r;
-#pragma unroll
-  for (int k = 0; k < VEC; ++k) r.v[k] = GnIo<T>::down(f[k]);
-  *reinterpret_cast<GnVec<T, VEC>*>(p) = r;
-}
-
-// NaN stays NaN (as torch's relu)
-template <int ACT>
-__device__ __forceinline__ float gn_act(float z) {
-  if constexpr (ACT == 1) return z <= 0.f ? 0.f : z;
-  if constexpr (ACT == 2) return z / (1.f + __expf(-z));
-  return z;
-}
-template <int ACT>
-__device__ __forceinline__ float gn_dact(float z, float g) {
-  if constexpr (ACT == 1) return z <= 0.f ? 0.f : g;
-  if constexpr (ACT == 2) {
-    const float s = 1.f / (1.f + __expf(-z));
-    return g * (s * (1.f + z * (1.f - s)));
-  }
-  return g;
-}
-
 // Block geometry: cols = C / VEC channel vectors; CW of them side by side, R pixel rows at once.
 struct GnGeo {
   int cols, CW, R;
@@ -94,19 +48,6 @@ struct GnGeo {
     R = GT / CW;
   }
 };
-
-// sum over the L (power of two) lanes of a segment, every lane gets it
-__device__ __forceinline__ float seg_sum(float v, int L) {
-  for (int o = L >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
-}
-
-// lanes that share one group's entries: the largest power of two <= min(64, entries)
-__device__ __forceinline__ int seg_lanes(int entries) {
-  int L = 1;
-  while (L < 64 && L * 2 <= entries) L <<= 1;
-  return L;
-}
 
 // ---------------------------------------------------------------- forward
 // part [N][chunks][G] = (mean, M2) over the chunk's pixels x cg channels
@@ -287,28 +228,6 @@ __global__ __launch_bounds__(GT) void gn_apply_kernel(const T* __restrict__ x, c
 }
 
 // --------------------------------------------------------------- backward
-// Where the activation's slope comes from: z of x alone, z of x and the residual, or the forward's bits.
-enum GnSlope { kOfX, kOfXRes, kOfMask };
-
-// dz of one vector; xc = x - mu
-template <int VEC, int ACT, int SLOPE>
-__device__ __forceinline__ void gn_dz(const float (&xc)[VEC], const float (&g)[VEC], const float (&r)[VEC],
-                                      unsigned bits, const float (&a)[VEC], const float (&be)[VEC], float (&dz)[VEC]) {
-#pragma unroll
-  for (int k = 0; k < VEC; ++k) {
-    if constexpr (ACT == 0) {
-      dz[k] = g[k];
-    } else if constexpr (SLOPE == kOfMask) {
-      dz[k] = (bits >> k) & 1 ? g[k] : 0.f;
-    } else {
-      // z in the forward's own steps (a = gamma rstd, one fma): its sign is the forward's
-      float z = fmaf(xc[k], a[k], be[k]);
-      if constexpr (SLOPE == kOfXRes) z += r[k];
-      dz[k] = gn_dact<ACT>(z, g[k]);
-    }
-  }
-}
-
 // cpart [rows of (n, chunk)][2][C] = sums over the chunk's pixels of dz and dz xhat (per channel);
 // gpart [N][chunks][G] = their gamma-weighted sums over the group
 template <typename T, int VEC, int ACT, int SLOPE>
@@ -598,6 +517,9 @@ long long gn_bwd_workspace_floats(int N, int HW, int C, int G, int esize) {
 
 int gn_fwd_launch(const GnArgs& a, hipStream_t st) {
   if (!gn_args_ok(a)) return 1;
+  GnOne one;
+  if (gn_one_plan(a.N, a.HW, a.C, a.G, a.esize, gn_align({a.x, a.res, a.out}), false, one))
+    return gn_one_fwd(a, one, st);
   const GnPlan p = gn_plan(a.N, a.HW, a.C, a.esize, gn_align({a.x, a.res, a.out}), kFwdBlocks);
   if (a.mask && p.vec * a.esize != 16) return 2;  // one byte per 16-byte vector
   float2* part = reinterpret_cast<float2*>(a.ws);
@@ -629,13 +551,16 @@ int gn_fwd_launch(const GnArgs& a, hipStream_t st) {
 
 int gn_bwd_launch(const GnArgs& a, hipStream_t st) {
   if (!gn_args_ok(a)) return 1;
-  const GnPlan p = gn_plan(a.N, a.HW, a.C, a.esize, gn_align({a.x, a.res, a.dout, a.dx, a.dres}), kBwdBlocks);
+  const uintptr_t align = gn_align({a.x, a.res, a.dout, a.dx, a.dres});
+  const GnPlan p = gn_plan(a.N, a.HW, a.C, a.esize, align, kBwdBlocks);
   if (a.mask && p.vec * a.esize != 16) return 2;
-  const long long rows = (long long)a.N * p.chunks;
+  GnOne one;
+  const bool in_one = (!a.res || a.act == 0) && gn_one_plan(a.N, a.HW, a.C, a.G, a.esize, align, a.act == 2, one);
+  const long long rows = in_one ? a.N : (long long)a.N * p.chunks;
   float* cpart = a.ws;
   float2* gpart = reinterpret_cast<float2*>(a.ws + rows * 2 * a.C);
   const size_t lds = gn_lds_stats(p, a.C), l2 = 2 * (size_t)a.G * sizeof(float);
-  const int rc = gn_dispatch_vec(a.esize, p.vec, [&](auto t, auto vec) {
+  const int rc = in_one ? gn_one_bwd(a, one, cpart, st) : gn_dispatch_vec(a.esize, p.vec, [&](auto t, auto vec) {
     using T = decltype(t);
     constexpr int V = decltype(vec)::value;
     return gn_dispatch_act(a.act, a.res != nullptr, a.mask != nullptr, [&](auto act, auto slope) {

@@ -106,6 +106,34 @@ def test_activations(act, with_res, dtype):
     _check(x, gn, res if with_res else None, dy, act)
 
 
+# samples whose groups fit a block's registers: a few and many pixels a thread, threads without any, groups of
+# 2 channels to all of a block's, one pixel
+ONE = [(64, (28, 28), 32, 4), (40, (27, 29), 64, 8), (300, (40, 43), 32, 16), (2, (14, 14), 256, 1), (3, (13,), 512, 8),
+       (260, (1,), 64, 32), (257, (56, 57), 32, 4)]
+
+
+@pytest.mark.parametrize("act,with_res", [("none", True), ("relu", False), ("relu", True), ("silu", False)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n,sp,c,groups", ONE)
+def test_in_registers(n, sp, c, groups, dtype, act, with_res):
+    x, gn, res, dy = _case(n, sp, c, groups, dtype, seed=20)
+    _check(x, gn, res if with_res else None, dy, act)
+
+
+@pytest.mark.parametrize("n,sp,c,groups", ONE + [(1, (130, 130), 16, 4), (4, (56, 56), 64, 32), (5, (31, 33), 10, 5)])
+def test_large_mean_everywhere(n, sp, c, groups):
+    g = torch.Generator().manual_seed(21)
+    x = (torch.randn(n, *sp, c, generator=g) + 1000.0).cuda()
+    x.view(n, -1, c)[:, 0] += 300.0                        # the first pixel is no guide to the mean
+    gn = torch.nn.GroupNorm(groups, c).cuda()
+    out = OF.group_norm_act(x, gn, act="none")
+    ref = _ref(x, None, gn.weight.detach(), gn.bias.detach(), x, groups, gn.eps, "none")[0]
+    # x - mean carries the mean's rounding and the last sums', each up to 1300 * 2^-24 for a few of them; a thread's
+    # sums about a shift 300 off lose up to 64 of their steps
+    rstd = _ref(x, None, gn.weight.detach(), gn.bias.detach(), x, groups, gn.eps, "none")[7].amax()
+    assert (out.double() - ref).abs().max() <= 128 * U32 * 1300 * rstd * (1 + ref.abs().max())
+
+
 @pytest.mark.parametrize("offset", [1, 2, 4])
 def test_unaligned_storage(offset):
     # a view that starts 2, 4 or 8 bytes into its storage: narrower loads, same values
