@@ -49,12 +49,37 @@ struct GnGeo {
   }
 };
 
+// lanes for one value a chunk (at most kMaxChunks of them)
+constexpr int kMaxChunks = 64;
+__device__ __forceinline__ int chunk_lanes(int chunks) {
+  int L = 1;
+  while (L < chunks) L <<= 1;
+  return L;
+}
+// f(g, part[lane][g] or 0) for every group, by L lanes each; the loads of eight rounds are under way at once
+template <typename F>
+__device__ __forceinline__ void join_chunks(const float2* part, int chunks, int G, int L, F&& f) {
+  const int lane = threadIdx.x & (L - 1), step = GT / L;
+  for (int g0 = threadIdx.x / L; g0 < G; g0 += 8 * step) {
+    float2 t[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int g = g0 + k * step;
+      t[k] = lane < chunks && g < G ? part[(size_t)lane * G + g] : make_float2(0.f, 0.f);
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (g0 + k * step < G) f(g0 + k * step, t[k]);
+  }
+}
+
 // ---------------------------------------------------------------- forward
 // part [N][chunks][G] = (mean, M2) over the chunk's pixels x cg channels
 template <typename T, int VEC>
 __global__ __launch_bounds__(GT) void gn_stats_kernel(const T* __restrict__ x, float2* __restrict__ part, int HW,
                                                       int C, int G, int chunks, int P) {
   extern __shared__ float lds[];  // [R][C] means, [R][C] M2
+  __shared__ float lc[GT];        // pixels of a slot
   const GnGeo geo(C, VEC);
   const int n = blockIdx.x / chunks, ch = blockIdx.x - n * chunks;
   const int p0 = ch * P, np = min(P, HW - p0);
@@ -64,90 +89,97 @@ __global__ __launch_bounds__(GT) void gn_stats_kernel(const T* __restrict__ x, f
   float* l2 = lds + geo.R * C;
   if (row < geo.R) {
     for (int col = tc; col < geo.cols; col += geo.CW) {
-      float mean[VEC], m2[VEC];
+      float* lmc = lm + row * C + col * VEC;  // this thread's mean and M2 so far: LDS, to leave registers
+      float* l2c = l2 + row * C + col * VEC;
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) mean[k] = m2[k] = 0.f;
+      for (int k = 0; k < VEC; ++k) lmc[k] = l2c[k] = 0.f;
       int cnt = 0;
       const T* xc = xb + col * VEC;
       for (int p = row; p < np;) {
-        float sh[VEC], s1[VEC], s2[VEC], v[GU][VEC];
+        float sh[VEC], s1[VEC], s2[VEC];
+        GnVec<T, VEC> v[GU];
         const int have = min(kSeg, (np - p + geo.R - 1) / geo.R);  // pixels of this segment
-        const int first = min(GU, have);
-#pragma unroll
-        for (int u = 0; u < GU; ++u) gn_load<T, VEC>(xc + (size_t)(p + min(u, first - 1) * geo.R) * C, v[u]);
-        const float w0 = 1.f / first;
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) {
-          float t = v[0][k];
-#pragma unroll
-          for (int u = 1; u < GU; ++u) t += u < first ? v[u][k] : 0.f;
-          sh[k] = t * w0;
-          s1[k] = s2[k] = 0.f;
-#pragma unroll
-          for (int u = 0; u < GU; ++u) {
-            const float d = u < first ? v[u][k] - sh[k] : 0.f;
-            s1[k] += d;
-            s2[k] = fmaf(d, d, s2[k]);
-          }
-        }
-        int i = first;
-        for (; i + GU <= have; i += GU) {
-#pragma unroll
-          for (int u = 0; u < GU; ++u) gn_load<T, VEC>(xc + (size_t)(p + (i + u) * geo.R) * C, v[u]);
+        auto batch = [&](int i) {  // pixels i .. of the segment, its last one again past the end
 #pragma unroll
           for (int u = 0; u < GU; ++u)
+            v[u] = *reinterpret_cast<const GnVec<T, VEC>*>(xc + (size_t)(p + min(i + u, have - 1) * geo.R) * C);
+        };
+        auto add = [&](int i) {
+#pragma unroll
+          for (int u = 0; u < GU; ++u) {
+            const float w = i + u < have ? 1.f : 0.f;
 #pragma unroll
             for (int k = 0; k < VEC; ++k) {
-              const float d = v[u][k] - sh[k];
+              const float d = (GnIo<T>::up(v[u].v[k]) - sh[k]) * w;
               s1[k] += d;
               s2[k] = fmaf(d, d, s2[k]);
             }
-        }
-        for (; i < have; ++i) {
-          gn_load<T, VEC>(xc + (size_t)(p + i * geo.R) * C, v[0]);
-#pragma unroll
-          for (int k = 0; k < VEC; ++k) {
-            const float d = v[0][k] - sh[k];
-            s1[k] += d;
-            s2[k] = fmaf(d, d, s2[k]);
           }
+        };
+        batch(0);
+        const float w0 = 1.f / min(GU, have);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+          float t = GnIo<T>::up(v[0].v[k]);
+#pragma unroll
+          for (int u = 1; u < GU; ++u) t += u < have ? GnIo<T>::up(v[u].v[k]) : 0.f;
+          sh[k] = t * w0;
+          s1[k] = s2[k] = 0.f;
+        }
+        add(0);
+        for (int i = GU; i < have; i += GU) {
+          batch(i);
+          add(i);
         }
         const float in = 1.f / have, w = (float)have / (cnt + have), nn = (float)cnt * w;
 #pragma unroll
         for (int k = 0; k < VEC; ++k) {
-          const float dm = s1[k] * in, q = fmaxf(s2[k] - s1[k] * dm, 0.f), d = sh[k] + dm - mean[k];
-          mean[k] += d * w;
-          m2[k] += (s2[k] != s2[k] ? s2[k] : q) + d * d * nn;  // fmaxf drops a NaN
+          const float dm = s1[k] * in, q = fmaxf(s2[k] - s1[k] * dm, 0.f), d = sh[k] + dm - lmc[k];
+          lmc[k] += d * w;
+          l2c[k] += (s2[k] != s2[k] ? s2[k] : q) + d * d * nn;  // fmaxf drops a NaN
         }
         cnt += have;
         p += have * geo.R;
       }
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) {
-        lm[row * C + col * VEC + k] = mean[k];
-        l2[row * C + col * VEC + k] = m2[k];
-      }
     }
   }
   __syncthreads();
-  // join the R x cg triples of a group
-  const int cg = C / G, ent = geo.R * cg;
+  // The triples of a channel first: its rows s, s + S, ..  (64 x 112 x 112 x 64 takes 28 us; 43 with all R x cg
+  // triples of a group joined at once, which leaves many groups to few waves, one after the other.)
+  const int S = C < GT ? GT / C : 1;
+  for (int e = tid; e < S * C; e += GT) {
+    const int s = e / C, c = e - s * C;
+    float cnt = 0.f, t = 0.f, q = 0.f;
+    for (int r = s; r < geo.R; r += S) {
+      const float nr = (float)((np - r + geo.R - 1) / geo.R);  // pixels of row r (0 when np <= r)
+      cnt += nr;
+      t += nr * lm[r * C + c];
+    }
+    const float mu = t / fmaxf(cnt, 1.f);
+    for (int r = s; r < geo.R; r += S) {
+      const float nr = (float)((np - r + geo.R - 1) / geo.R), d = lm[r * C + c] - mu;
+      q += nr > 0.f ? l2[r * C + c] + nr * d * d : 0.f;
+    }
+    lm[s * C + c] = mu;  // row s is this thread's alone
+    l2[s * C + c] = q;
+    if (c == 0) lc[s] = cnt;
+  }
+  __syncthreads();
+  const int cg = C / G, ent = S * cg;
   const int L = seg_lanes(ent), lane = tid & (L - 1);
   const float inv = 1.f / ((float)np * cg);
   for (int g = tid / L; g < G; g += GT / L) {
-    float s = 0.f;
+    float t = 0.f;
     for (int e = lane; e < ent; e += L) {
-      const int r = e / cg, c = e - r * cg;
-      const int nr = (np - r + geo.R - 1) / geo.R;  // pixels of row r (0 when np <= r)
-      s += nr * lm[r * C + g * cg + c];
+      const int s = e / cg, c = e - s * cg;
+      t += lc[s] * lm[s * C + g * cg + c];
     }
-    const float mu = seg_sum(s, L) * inv;
+    const float mu = seg_sum(t, L) * inv;
     float q = 0.f;
     for (int e = lane; e < ent; e += L) {
-      const int r = e / cg, c = e - r * cg;
-      const int nr = (np - r + geo.R - 1) / geo.R;
-      const float d = lm[r * C + g * cg + c] - mu;
-      q += l2[r * C + g * cg + c] + nr * d * d;
+      const int s = e / cg, c = e - s * cg;
+      const float n = lc[s], d = lm[s * C + g * cg + c] - mu;
+      q += n > 0.f ? l2[s * C + g * cg + c] + n * d * d : 0.f;
     }
     q = seg_sum(q, L);
     if (lane == 0) part[((size_t)n * chunks + ch) * G + g] = make_float2(mu, q);
@@ -167,26 +199,17 @@ __global__ __launch_bounds__(GT) void gn_apply_kernel(const T* __restrict__ x, c
   const int n = blockIdx.x / chunks, ch = blockIdx.x - n * chunks;
   const int tid = threadIdx.x, cg = C / G;
   {
-    const float2* pn = part + (size_t)n * chunks * G;
-    const int L = seg_lanes(chunks), lane = tid & (L - 1);
-    const float total = (float)HW * cg;
-    for (int g = tid / L; g < G; g += GT / L) {
-      float s = 0.f;
-      for (int c = lane; c < chunks; c += L) s += (float)min(P, HW - c * P) * pn[(size_t)c * G + g].x;
-      const float mu = seg_sum(s, L) / HW;
-      float q = 0.f;
-      for (int c = lane; c < chunks; c += L) {
-        const float2 t = pn[(size_t)c * G + g];
-        const float d = t.x - mu;
-        q += t.y + (float)min(P, HW - c * P) * cg * d * d;
-      }
-      const float rstd = rsqrtf(seg_sum(q, L) / total + eps);
+    const int L = chunk_lanes(chunks), lane = tid & (L - 1);
+    const float np = lane < chunks ? (float)min(P, HW - lane * P) : 0.f, total = (float)HW * cg;
+    join_chunks(part + (size_t)n * chunks * G, chunks, G, L, [&](int g, const float2& t) {
+      const float mu = seg_sum(np * t.x, L) / HW, d = t.x - mu;
+      const float rstd = rsqrtf(seg_sum(np > 0.f ? t.y + np * cg * d * d : 0.f, L) / total + eps);
       if (lane == 0) {
         lds[g] = mu;
         lds[G + g] = rstd;
         if (ch == 0) stats[(size_t)n * G + g] = make_float2(mu, rstd);
       }
-    }
+    });
   }
   __syncthreads();
   const int row = tid / geo.CW, tc = tid - row * geo.CW;
@@ -319,23 +342,15 @@ __global__ __launch_bounds__(GT) void gn_bwd_apply_kernel(
   const int n = blockIdx.x / chunks, ch = blockIdx.x - n * chunks;
   const int tid = threadIdx.x, cg = C / G;
   {
-    const float2* pn = gpart + (size_t)n * chunks * G;
-    const int L = seg_lanes(chunks), lane = tid & (L - 1);
+    const int L = chunk_lanes(chunks), lane = tid & (L - 1);
     const float inv = 1.f / ((float)HW * cg);
-    for (int g = tid / L; g < G; g += GT / L) {
-      float a = 0.f, b = 0.f;
-      for (int c = lane; c < chunks; c += L) {
-        const float2 t = pn[(size_t)c * G + g];
-        a += t.x;
-        b += t.y;
-      }
-      a = seg_sum(a, L);
-      b = seg_sum(b, L);
+    join_chunks(gpart + (size_t)n * chunks * G, chunks, G, L, [&](int g, const float2& t) {
+      const float a = seg_sum(t.x, L), b = seg_sum(t.y, L);
       if (lane == 0) {
         lds[g] = a * inv;
         lds[G + g] = b * inv;
       }
-    }
+    });
   }
   __syncthreads();
   const int row = tid / geo.CW, tc = tid - row * geo.CW;
@@ -415,7 +430,7 @@ int gn_vec(int C, int esize, uintptr_t align) {
 // Chunks of about N HW / blocks pixels: 2,048 blocks forward, 4,096 backward (256 x 56 x 56 x 256 bf16:
 // 117 us + 242 us against 124 + 243 for stats and apply forward, 186 + 320 against 225 + 347 backward), but
 // at least 48 KiB each and 4 pixels a thread, for a block joins all of its sample's partials first (64 x 112 x
-// 112 x 64: 40 us in chunks of 49 KiB, 63 in 25), and at most 64 a sample.
+// 112 x 64 forward: 83 us in chunks of 49 KiB, 109 in 25), and at most 64 a sample.
 GnPlan gn_plan(int N, int HW, int C, int esize, uintptr_t align, int blocks) {
   GnPlan p;
   p.vec = gn_vec(C, esize, align);
@@ -426,7 +441,7 @@ GnPlan gn_plan(int N, int HW, int C, int esize, uintptr_t align, int blocks) {
   // the floor on the bytes holds where the device is full all the same (512 blocks of it)
   const long long floor_px = (48 << 10) / ((long long)C * esize);
   if ((long long)N * HW / 512 >= floor_px) per = std::max(per, floor_px);
-  per = std::max<long long>({per, (HW + 63) / 64, (long long)p.R * GU});
+  per = std::max<long long>({per, (HW + kMaxChunks - 1) / kMaxChunks, (long long)p.R * GU});
   if (per > HW) per = HW;
   p.P = (int)per;
   p.chunks = (HW + p.P - 1) / p.P;
