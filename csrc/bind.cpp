@@ -797,7 +797,8 @@ static pmd::GnArgs gn_args(const Tensor& x, const c10::optional<Tensor>& res, co
   TORCH_CHECK(groups >= 1 && C % groups == 0, "group_norm: ", C, " channels do not split into ", groups, " groups");
   int64_t hw = 1;
   for (int64_t d = 1; d < x.dim() - 1; ++d) hw *= x.size(d);
-  TORCH_CHECK(N < (1ll << 25) && hw < (1ll << 31), "group_norm: too many samples or pixels");
+  // a block or more for each sample, of up to 512 threads: a launch has fewer than 2^32 threads
+  TORCH_CHECK(N <= (1ll << 23) && hw < (1ll << 31), "group_norm: at most 2^23 samples of 2^31 - 1 pixels");
   TORCH_CHECK(act >= 0 && act <= 2, "group_norm: unknown activation");
   a.N = (int)N; a.HW = (int)hw; a.C = (int)C; a.G = (int)groups; a.act = (int)act; a.eps = (float)eps;
   a.x = x.data_ptr();
@@ -883,6 +884,8 @@ static pmd::LxShape lx_shape(int64_t N, int64_t D, bool x_f32, const Tensor& w, 
               "linear_xent: target must be int64 [N]");
   TORCH_CHECK(N <= (1 << 24) && w.size(0) >= 1 && w.size(0) <= (1 << 30) && D >= 1 && D <= (1 << 21) - 8,
               "linear_xent: at most 2^24 rows, 2^30 classes, 2^21 - 8 features");
+  // 512 threads for 2^16 logits: a launch has fewer than 2^32 threads
+  TORCH_CHECK(N * w.size(0) <= (1ll << 38), "linear_xent: at most 2^38 logits, got ", N, " x ", w.size(0));
   pmd::LxShape s{};
   s.N = (int)N; s.V = (int)w.size(0); s.D = (int)D;
   s.planes = bf16_products || (!x_f32 && w16) ? 1 : 3;

@@ -486,7 +486,7 @@ int gn_allow_lds(K kernel, size_t bytes) {
 
 bool gn_args_ok(const GnArgs& a) {
   return a.N >= 1 && a.HW >= 1 && a.C >= 1 && a.C <= kGnMaxChannels && a.G >= 1 && a.C % a.G == 0 &&
-         (a.esize == 2 || a.esize == 4) && a.act >= 0 && a.act <= 2 && (long long)a.N * 64 < (1ll << 31);
+         (a.esize == 2 || a.esize == 4) && a.act >= 0 && a.act <= 2 && a.N <= (1 << 23);
 }
 
 uintptr_t gn_align(std::initializer_list<const void*> ps) {

@@ -422,7 +422,7 @@ bool gn_one_plan(int N, int HW, int C, int G, int esize, uintptr_t align, bool s
       if (CB % cg || C % CB) continue;
       if (k == 25 && (silu_bwd || (long long)N * (C / CB) < 256)) continue;
       for (int nt : {128, 256, 512})
-        if (nt >= CB && HW <= (long long)k * (nt / cols)) {
+        if (nt >= CB && HW <= (long long)k * (nt / cols) && (long long)N * (C / CB) * nt < (1ll << 32)) {
           o = GnOne{CB, nt, k};
           return true;
         }

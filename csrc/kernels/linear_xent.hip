@@ -868,7 +868,7 @@ void lx_prep(const void* src, bool f32, int rows, int cols, bf16_t* dst, int ld,
 
 bool lx_ok(const LxShape& s) {
   return s.N >= 1 && s.V >= 1 && s.D >= 1 && (s.planes == 1 || s.planes == 3) && s.D <= kGemmMaxLd - 8 &&
-         s.V <= (1 << 30) && s.N <= (1 << 24);
+         s.V <= (1 << 30) && s.N <= (1 << 24) && (long long)s.N * s.V <= (1ll << 38);
 }
 
 template <int PL>

@@ -239,6 +239,32 @@ def test_refusals_gpu():
     big = torch.nn.GroupNorm(1, 16392).cuda()
     with pytest.raises(RuntimeError, match="channels"):
         OF.group_norm_act(torch.zeros(1, 16392, device="cuda"), big)
+    with pytest.raises(RuntimeError, match="samples"):
+        OF.group_norm_act(torch.zeros(2 ** 23 + 1, 4, device="cuda"), torch.nn.GroupNorm(2, 4).cuda())
+
+
+@pytest.mark.parametrize("n,c", [(2 ** 23, 8), (2 ** 20, 64)])
+def test_many_samples(n, c):
+    # a pixel a sample: more samples than one grid's threads would allow at 512 a block
+    x = torch.randn(n, c, device="cuda", dtype=torch.bfloat16)
+    gn = torch.nn.GroupNorm(2, c).cuda()
+    with torch.no_grad():
+        out = OF.group_norm_act(x, gn, act="none")
+    rows = torch.tensor([0, 1, n // 2, n - 2, n - 1], device="cuda")
+    ref = _ref(x[rows], None, gn.weight.detach(), gn.bias.detach(), x[rows], 2, gn.eps, "none")[0]
+    # outputs of up to 2^3: half a bf16 step, and fp32 errors far below one
+    assert ((out[rows].double() - ref).abs() <= 2.0 ** -8 * ref.abs() + 2.0 ** -14).all()
+
+
+@pytest.mark.parametrize("act,with_res", [("relu", True), ("silu", True), ("relu", False)])
+def test_backward_twice_over_a_retained_graph(act, with_res):
+    for shape in ((4, (56, 56), 64, 32), (6, (14, 14), 64, 32)):
+        x, gn, res, dy = _case(*shape, torch.bfloat16, seed=22)
+        xg = x.clone().requires_grad_(True)
+        out = OF.group_norm_act(xg, gn, residual=res if with_res else None, act=act)
+        a = torch.autograd.grad(out, [xg, gn.weight, gn.bias], dy, retain_graph=True)
+        b = torch.autograd.grad(out, [xg, gn.weight, gn.bias], dy)
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
 
 
 @pytest.mark.parametrize("act", ["none", "relu", "silu"])

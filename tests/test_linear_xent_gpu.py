@@ -298,6 +298,52 @@ def test_arena_gradients_accumulate():
     flat.zero_grad()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_backward_twice_over_a_retained_graph(dtype):
+    x, lin, t = _case(130, 72, 900, dtype, seed=23)
+    loss, _ = OF.linear_cross_entropy(x, lin, t)
+    a = torch.autograd.grad(loss, [x, lin.weight, lin.bias], retain_graph=True)
+    b = torch.autograd.grad(loss, [x, lin.weight, lin.bias])
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def test_too_many_logits_are_refused():
+    x = torch.zeros(2 ** 24, 1, device="cuda", dtype=torch.bfloat16)
+    lin = torch.nn.Linear(1, 2 ** 14 + 1, bias=False, device="cuda", dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="2\\^38 logits"):
+        OF.linear_cross_entropy(x, lin, torch.zeros(2 ** 24, dtype=torch.int64, device="cuda"))
+
+
+@pytest.mark.parametrize("want", [False, True])
+def test_captured_step_beside_an_eager_one(want):
+    """A forward and backward captured on its own leaves, replayed between eager calls of other sizes."""
+    x, lin, t = _case(96, 64, 500, torch.bfloat16, seed=24)
+    leaves = [x, lin.weight] + ([lin.bias] if want else [])
+    lin.bias.requires_grad_(want)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        for _ in range(2):
+            torch.autograd.grad(OF.linear_cross_entropy(x, lin, t)[0], leaves)
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        loss, correct = OF.linear_cross_entropy(x, lin, t)
+        got = torch.autograd.grad(loss, leaves)
+    x2, lin2, t2 = _case(70, 48, 1300, torch.bfloat16, seed=25)
+    for i in range(4):
+        with torch.no_grad():
+            x.copy_(torch.randn(x.shape, generator=torch.Generator().manual_seed(i)).to(x.dtype))
+        graph.replay()
+        torch.autograd.grad(OF.linear_cross_entropy(x2, lin2, t2)[0], [x2])
+        torch.cuda.synchronize()
+        l2, c2 = OF.linear_cross_entropy(x, lin, t)
+        ref = torch.autograd.grad(l2, leaves)
+        assert torch.equal(loss, l2) and torch.equal(correct, c2)
+        assert all(torch.equal(p, q) for p, q in zip(got, ref))
+
+
 def test_refusals_gpu():
     x, lin, t = _case(4, 8, 6, torch.float32, ignored=False)
     with pytest.raises(RuntimeError, match="bf16 or fp32"):
