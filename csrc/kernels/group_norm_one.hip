@@ -73,7 +73,7 @@ __device__ __forceinline__ void gn_clear(Raw& r, int k, bool keep) {
 
 // A block's place: sample n, channels c0 .. c0 + CB, this thread's vector tc of them and its first pixel row
 struct GnSpot {
-  int n, c0, tc, row, R, CB, have;
+  int n, c0, tc, row, R, CB, each, more, have;
   __device__ __forceinline__ GnSpot(int HW, int C, int CB_, int VEC) : CB(CB_) {
     const int nb = C / CB, b = xcd_remap(blockIdx.x, gridDim.x);  // neighbours share lines of 128 bytes
     n = b / nb;
@@ -82,12 +82,12 @@ struct GnSpot {
     R = blockDim.x / cols;
     row = threadIdx.x / cols;
     tc = threadIdx.x - row * cols;
-    have = max(0, (HW - row + R - 1) / R);
+    each = HW / R;
+    more = HW - each * R;
+    have = pixels(row);
   }
+  __device__ __forceinline__ int pixels(int r) const { return each + (r < more ? 1 : 0); }  // of a row of threads
 };
-
-// pixels of rows s, s + S, .. below R
-__device__ __forceinline__ float rows_pixels(int r, int R, int HW) { return (float)max(0, (HW - r + R - 1) / R); }
 
 template <typename T, int VEC, int ACT, bool RES, bool MASK, int K>
 __global__ __launch_bounds__(kOneThreads) void gn_one_fwd_kernel(const T* __restrict__ x, const T* __restrict__ res,
@@ -160,13 +160,13 @@ __global__ __launch_bounds__(kOneThreads) void gn_one_fwd_kernel(const T* __rest
     const int c = tid % CB, s = tid / CB;
     float cnt = 0.f, t = 0.f, q = 0.f;
     for (int r = s; r < at.R; r += S) {
-      const float nr = rows_pixels(r, at.R, HW);
+      const float nr = (float)at.pixels(r);
       cnt += nr;
       t += nr * lm[r * CB + c];
     }
     const float mu = t / fmaxf(cnt, 1.f);
     for (int r = s; r < at.R; r += S) {
-      const float nr = rows_pixels(r, at.R, HW), d = lm[r * CB + c] - mu;
+      const float nr = (float)at.pixels(r), d = lm[r * CB + c] - mu;
       q += nr > 0.f ? l2[r * CB + c] + nr * d * d : 0.f;
     }
     sm[tid] = mu;
@@ -474,7 +474,9 @@ int gn_one_bwd(const GnArgs& a, const GnOne& o, float* cpart, hipStream_t st) {
     auto typed = [&](auto t) {
       typedef std::integral_constant<int, kOfX> X;
       if (a.act == 0) return run(t, std::integral_constant<int, 0>{}, X{});
-      if (a.act == 2) return run(t, std::integral_constant<int, 2>{}, X{});
+      if constexpr (K <= 13)  // gn_one_plan
+        if (a.act == 2) return run(t, std::integral_constant<int, 2>{}, X{});
+      if (a.act == 2) return 2;
       if (a.mask) return run(t, std::integral_constant<int, 1>{}, std::integral_constant<int, kOfMask>{});
       return run(t, std::integral_constant<int, 1>{}, X{});
     };
