@@ -131,6 +131,11 @@ class Muon(FusedSGD):
             dict(params=rest, lr=rest_lr, momentum=rest_momentum, weight_decay=rest_weight_decay,
                  nesterov=rest_nesterov)], {})
         self.ns = (int(ns_steps), tuple(float(c) for c in ns_coeffs), float(eps))
+        # what the orthogonalisation refuses, it refuses here rather than in the middle of a step
+        if any(max(p.shape[0], p.numel() // p.shape[0]) > 2 ** 20 for p in mats):
+            raise ValueError("Muon: matrices of at most 2^20 rows and columns")
+        one = torch.zeros(1, 1, device=self.flat.device)
+        prims_for(one).newton_schulz_([one], [one.clone()], *self.ns, [1.0])
         self.momentum_arena = torch.zeros_like(self.flat.param_arena)
         self.flat.companions.append(self.momentum_arena)   # follows arena relayouts
         self.update_arena = torch.zeros_like(self.flat.param_arena)   # written and read within a step

@@ -149,6 +149,13 @@ def test_muon_groups_schedule_and_refusals():
     only.step()
 
 
+def test_muon_refuses_matrices_past_its_sides():
+    from pytorch_multiprocessing_distributed_amd.engine.optim import Muon
+    lin = torch.nn.Linear(2, 2 ** 20 + 1, bias=False)
+    with pytest.raises(ValueError, match="at most 2\\^20"):
+        Muon(lin, matrices=[lin.weight])
+
+
 def test_muon_without_matrices_is_sgd():
     a, b = _small(), _small()
     oa = Muon(a, matrices=[], rest_lr=0.1, rest_momentum=0.9, rest_weight_decay=1e-4)

@@ -107,6 +107,14 @@ def _steps(graph, m0, batches):
     return torch.stack(rows), opt.flat.param_arena.clone(), opt.momentum_arena.clone()
 
 
+def test_muon_refuses_before_any_step():
+    from pytorch_multiprocessing_distributed_amd.engine.optim import Muon
+    for kw, match in ((dict(ns_coeffs=(50.0, 0.0, 0.0)), "range"), (dict(ns_steps=65), "steps"),
+                      (dict(eps=-1.0), "eps")):
+        with pytest.raises(RuntimeError, match=match):
+            Muon(torch.nn.Conv2d(8, 8, 3).cuda(), **kw)
+
+
 def test_captured_step_is_bit_exact():
     from pytorch_multiprocessing_distributed_amd.models import build_model
     from pytorch_multiprocessing_distributed_amd.ops import functional as OF
