@@ -818,17 +818,32 @@ struct NsScales {
 
 // Powers of two for every step.  [0, hi] holds the singular values, so hi bounds the entries of X,
 // hi^2 those of S and max |b t + c t^2| over t <= hi^2 those of P; each is scaled to at most 2^15
-// (fp16 ends at 65,504: a factor of two covers the bound's sampling and the roundings).
+// (fp16 ends at 65,504: a factor of two covers the roundings).  The largest values lie at the ends or
+// where the derivative vanishes: b + 2 c t = 0 for P, a + 3 b w + 5 c w^2 = 0 (w = v^2) for the next X.
 bool ns_scales(int steps, float a, float b, float c, NsScales* out) {
   if (!std::isfinite(a) || !std::isfinite(b) || !std::isfinite(c)) return false;
   double hi = 1.0;
   auto pow2 = [](double bound) { return (float)std::ldexp(1.0, std::min(40, (int)std::floor(15.0 - std::log2(bound)))); };
   for (int k = 0; k < steps; ++k) {
     double mp = 1e-6, mx = 1e-6;
-    for (int i = 1; i <= 4096; ++i) {
-      const double v = hi * i / 4096, t = v * v;
-      mp = std::max(mp, std::fabs(b * t + c * t * t));
-      mx = std::max(mx, std::fabs(v * (a + b * t + c * t * t)));
+    const double end = hi * hi;
+    auto at_p = [&](double t) {
+      if (t > 0 && t <= end) mp = std::max(mp, std::fabs(t * ((double)b + (double)c * t)));
+    };
+    auto at_x = [&](double w) {
+      if (w > 0 && w <= end) mx = std::max(mx, std::fabs(std::sqrt(w) * ((double)a + w * ((double)b + (double)c * w))));
+    };
+    at_p(end);
+    at_x(end);
+    if (c != 0.f) {
+      at_p(-(double)b / (2.0 * c));
+      const double d = 9.0 * b * b - 20.0 * (double)a * c;
+      if (d >= 0) {
+        at_x((-3.0 * b + std::sqrt(d)) / (10.0 * c));
+        at_x((-3.0 * b - std::sqrt(d)) / (10.0 * c));
+      }
+    } else if (b != 0.f) {
+      at_x(-(double)a / (3.0 * b));
     }
     mp *= 1.01;
     mx *= 1.01;
