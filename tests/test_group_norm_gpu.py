@@ -109,7 +109,8 @@ def test_activations(act, with_res, dtype):
 # samples whose groups fit a block's registers: a few and many pixels a thread, threads without any, groups of
 # 2 channels to all of a block's, one pixel
 ONE = [(64, (28, 28), 32, 4), (40, (27, 29), 64, 8), (300, (40, 43), 32, 16), (2, (14, 14), 256, 1), (3, (13,), 512, 8),
-       (260, (1,), 64, 32), (257, (56, 57), 32, 4)]
+       (260, (1,), 64, 32), (257, (56, 57), 32, 4), (9, (10, 11), 40, 8), (5, (6, 7), 56, 8), (6, (20, 21), 120, 10),
+       (3, (9, 5), 24, 2), (4, (12, 11), 160, 16), (2, (7, 7), 224, 2)]
 
 
 @pytest.mark.parametrize("act,with_res", [("none", True), ("relu", False), ("relu", True), ("silu", False)])
