@@ -59,6 +59,7 @@ constexpr int kNormBlocks = 256;  // partial sums of a matrix's norm, at most
 struct NsCut {
   int kc;                                   // reduction of a Gram block
   int gram_small, poly_small, upd_small;    // 64-wide tiles for all
+  int gram_wide, poly_wide;                 // 192-wide tiles for all
   int upd_big;                              // 256-wide tiles for all
 };
 struct NsBlocks {
@@ -73,12 +74,12 @@ __host__ __device__ inline NsBlocks ns_blocks(int phase, int s, int l, const NsC
   } else if (phase == kStart) {
     b.blocks = (int)(cdiv(s, 64) * cdiv(lp, 64));
   } else if (phase == kGram || phase == kJoin) {
-    b.tile = c.gram_small ? 64 : t;
+    b.tile = c.gram_wide ? 192 : c.gram_small ? 64 : t;
     b.splits = (int)cdiv(l, c.kc);
     const int tiles = tri((int)cdiv(s, b.tile));
     b.blocks = phase == kGram ? tiles * b.splits : b.splits > 1 ? tiles * (b.tile * b.tile / 1024) : 0;
   } else if (phase == kPoly) {
-    b.tile = c.poly_small ? 64 : t;
+    b.tile = c.poly_wide ? 192 : c.poly_small ? 64 : t;
     b.blocks = tri((int)cdiv(s, b.tile));
   } else {
     b.tile = c.upd_big ? 256 : c.upd_small ? 64 : t;
@@ -286,7 +287,8 @@ __device__ __forceinline__ void for_rows(F&& f) {
   static_assert(G::MI % R == 0, "whole runs");
   f(std::integral_constant<int, 0>{}, std::integral_constant<int, R>{});
   if constexpr (G::MI > R) f(std::integral_constant<int, R>{}, std::integral_constant<int, R>{});
-  static_assert(G::MI <= 2 * R, "two runs");
+  if constexpr (G::MI > 2 * R) f(std::integral_constant<int, 2 * R>{}, std::integral_constant<int, R>{});
+  static_assert(G::MI <= 3 * R, "three runs");
 }
 
 // the tiles (m + 16 i, n + 16 j) of a matrix in two planes (zero outside [rows][cols])
@@ -306,7 +308,7 @@ __device__ __forceinline__ void load_planes(const unsigned short* p, long long p
 }
 
 // The kernels below take their tile per matrix: the grid of a group mixes 128- and 64-wide tiles (G1,
-// G2: 256 threads each), a group of large matrices runs on 256-wide ones alone (G1 = G2).
+// G2: 256 threads each), a group of large matrices runs on 192- or 256-wide ones alone (G1 = G2).
 template <class G1, class G2>
 constexpr int ns_lds() {
   return G1::LDS > G2::LDS ? G1::LDS : G2::LDS;
@@ -754,9 +756,13 @@ template <bool TB>
 using NsMidL = Gemm<128, 128, 2, 4, 64, 2, 2, false, TB, true>;
 template <bool TB>
 using NsSmallL = Gemm<64, 64, 2, 4, 64, 4, 2, false, TB, true>;
+// twelve waves, three to a SIMD: 222 us for a Gram product of 4,096 x 4,096 (four waves: 242)
+using NsWide = Gemm<192, 192, 4, 3, 32, 3, 2, false, false, true>;
 // f(G1, G2) with the tiles of a phase of so many blocks
 template <bool TB, typename F>
-void ns_with(bool latency, F&& f) {
+void ns_with(bool latency, F&& f, bool wide = false) {
+  if constexpr (!TB)
+    if (wide) return f(NsWide{}, NsWide{});
   if (latency) f(NsMidL<TB>{}, NsSmallL<TB>{});
   else f(NsMid<TB>{}, NsSmall<TB>{});
 }
@@ -806,6 +812,17 @@ NsPlan ns_plan(const NsMatrix* mats, int n) {
   // the Gram reduction is cut into pieces of kc (at least 256), for at most about 1,000 blocks in all
   // (ResNet-50's mixture: 58 us, and 20 for the join; 68 and 17 with 600 blocks)
   while (p.cut.kc < longest && blocks(kGram) > 1000) p.cut.kc += 64;
+  // The symmetric products on 192-wide tiles, one a compute unit, where their rounds take less than those of
+  // 128-wide ones, two a unit (a last round of at most 256 has the units to itself): 4,096 x 4,096 in 253 tiles
+  // takes 222 + 227 us (Gram and polynomial), in 528 285 + 292.
+  auto wide = [&](int phase, int& on) {
+    const long long b = blocks(phase), rest = b % 512;
+    const long long mid = (b / 512 * 2 + (rest > 256 ? 2 : rest > 0 ? 1 : 0)) * 128 * 128;
+    on = 1;
+    on = shortest > 192 && cdiv(blocks(phase), 256) * 192 * 192 < mid;
+  };
+  if (p.cut.kc >= longest) wide(kGram, p.cut.gram_wide);
+  wide(kPoly, p.cut.poly_wide);
   for (int ph = 0; ph < kPhases; ++ph) p.blocks[ph] = (int)blocks(ph);
   p.slab_stride = p.cut.gram_small ? 64 * 64 : 128 * 128;
   p.slab_floats = p.blocks[kJoin] ? (long long)p.blocks[kGram] * p.slab_stride : 0;
@@ -954,13 +971,13 @@ int ns_launch(const NsMatrix* mats, int n, bool f32, int steps, float a, float b
       ns_with<false>(p.blocks[kGram] <= kNsFew, [&](auto g1, auto g2) {
         hipLaunchKernelGGL((ns_gram_kernel<decltype(g1), decltype(g2)>), dim3(p.blocks[kGram]), dim3(g1.NT), 0, st, tab,
                            W, xb, p.cut.kc, gmul, slab, p.slab_stride);
-      });
+      }, p.cut.gram_wide);
       if (p.blocks[kJoin])
         hipLaunchKernelGGL(ns_join_kernel, dim3(p.blocks[kJoin]), dim3(256), 0, st, tab, W, slab, p.slab_stride, gmul);
       ns_with<false>(p.blocks[kPoly] <= kNsFew, [&](auto g1, auto g2) {
         hipLaunchKernelGGL((ns_poly_kernel<decltype(g1), decltype(g2)>), dim3(p.blocks[kPoly]), dim3(g1.NT), 0, st, tab,
                            W, b, c, 1.f / sc[k].s, sc[k].p);
-      });
+      }, p.cut.poly_wide);
       const bool last = k + 1 == steps;
       const NsStep u{a, 1.f / sc[k].x, 1.f / sc[k].p, last ? 1.f : sc[k + 1].x, beta, f, alpha_dev};
       auto update = [&](auto g1, auto g2) {

@@ -59,7 +59,8 @@ def test_against_fp64(m, n, dtype):
     _check(u, OF.newton_schulz(u))
 
 
-@pytest.mark.parametrize("m,n", [(2048, 2048), (1500, 5000)])
+# the last two: symmetric products on 192-wide tiles, the last row of tiles short and full
+@pytest.mark.parametrize("m,n", [(2048, 2048), (1500, 5000), (3990, 4100), (4224, 4224)])
 def test_large_tiles(m, n):
     u = _mat(m, n, seed=1)
     _check(u, OF.newton_schulz(u))
