@@ -7,7 +7,8 @@
 // The logits are never stored.  Forward: the product's epilogue reduces its tile to (max, sum of
 // exponentials, argmax) per row, one combine pass joins the column tiles, one block sums the rows.
 // When a backward will follow, the epilogue also keeps the exponentials it has at hand, about the
-// maximum of their row in the wave's columns, if they take at most kKeepBytes.
+// maximum of their row in the wave's columns, if they take at most kKeepBytes (with the weight's copy, where
+// it is not read in place).
 // Backward, per piece of the vocabulary: softmax - onehot is written in 16 bits (a piece holds at most
 // kPieceBytes, which the last-level cache keeps) and the two gradient products read it from there.  It
 // comes from the kept exponentials, times exp(their maximum - lse), in a pass bound by memory; or, past
@@ -770,7 +771,8 @@ LxPlan lx_plan(const LxShape& s, bool kept) {
   p.fwd_ct = (s.V + p.fwd_tile - 1) / p.fwd_tile;
   p.kshift = p.fwd_tile == 64 ? 5 : 6;
   p.ldk = up(s.V, 64);
-  p.keep = kept && s.N * (p.ldk + (p.ldk >> p.kshift) * 2) * (s.planes == 1 ? 2 : 4) <= kKeepBytes;
+  p.keep = kept && s.N * (p.ldk + (p.ldk >> p.kshift) * 2) * (s.planes == 1 ? 2 : 4) +
+                           (p.w_direct ? 0 : 2ll * s.planes * s.V * p.Dp) <= kKeepBytes;
   const int vp = up(s.V, 64);
   long long piece = kPieceBytes / (2ll * s.planes * s.N) / 256 * 256;
   if (piece < 1024) piece = 1024;
@@ -817,7 +819,7 @@ struct LxBuf {
 LxBuf lx_carve(const LxShape& s, const LxPlan& p, bool bwd, char* base, long long* bytes) {
   Carver c{base};
   LxBuf b{};
-  if (!p.w_direct) b.w = c.take<bf16_t>((long long)s.planes * s.V * p.Dp);
+  if (!p.w_direct && !p.keep) b.w = c.take<bf16_t>((long long)s.planes * s.V * p.Dp);
   if (!bwd) {
     const long long n = (long long)p.fwd_ct * s.N;
     b.pmax = c.take<float>(n);
@@ -838,6 +840,7 @@ LxBuf lx_carve(const LxShape& s, const LxPlan& p, bool bwd, char* base, long lon
 struct LxKept {  // what a forward keeps for its backward
   void* e;
   float *ref, *tlogit;
+  bf16_t* w;             // the weight laid out, unless it is read in place
 };
 LxKept lx_kept(const LxShape& s, const LxPlan& p, void* base, long long* bytes) {
   Carver c{static_cast<char*>(base)};
@@ -845,6 +848,7 @@ LxKept lx_kept(const LxShape& s, const LxPlan& p, void* base, long long* bytes) 
   k.e = c.take<char>(s.N * p.ldk * (s.planes == 1 ? 2 : 4));
   k.ref = c.take<float>((long long)s.N * (up(s.V, p.fwd_tile) >> p.kshift));
   k.tlogit = c.take<float>(s.N);
+  if (!p.w_direct) k.w = c.take<bf16_t>((long long)s.planes * s.V * p.Dp);
   *bytes = c.off;
   return k;
 }
@@ -877,7 +881,10 @@ int lx_fwd_t(const LxShape& s, const LxIo& io, hipStream_t st) {
   long long bytes;
   LxBuf b = lx_carve(s, p, false, static_cast<char*>(io.ws), &bytes);
   const LxKept kept = lx_kept(s, p, io.kept, &bytes);
-  if (io.kept) b.tlogit = kept.tlogit;
+  if (io.kept) {
+    b.tlogit = kept.tlogit;
+    b.w = kept.w;
+  }
   b.x = static_cast<bf16_t*>(io.xp);
   lx_prep<PL>(io.x, s.x_f32, s.N, s.D, b.x, p.Dp, io.target, io.ignore, st);
   if (!p.w_direct) lx_prep<PL>(io.w, s.w_f32, s.V, s.D, b.w, p.Dp, nullptr, 0, st);
@@ -914,8 +921,8 @@ int lx_bwd_t(const LxShape& s, const LxIo& io, hipStream_t st) {
   LxBuf b = lx_carve(s, p, true, static_cast<char*>(io.ws), &bytes);
   b.x = static_cast<bf16_t*>(io.xp);  // the forward's
   const LxKept kept = lx_kept(s, p, io.kept, &bytes);
-  if (!p.w_direct && (!io.kept || io.dx)) lx_prep<PL>(io.w, s.w_f32, s.V, s.D, b.w, p.Dp, nullptr, 0, st);
-  const bf16_t* wbase = p.w_direct ? static_cast<const bf16_t*>(io.w) : b.w;
+  if (!p.w_direct && !io.kept) lx_prep<PL>(io.w, s.w_f32, s.V, s.D, b.w, p.Dp, nullptr, 0, st);
+  const bf16_t* wbase = p.w_direct ? static_cast<const bf16_t*>(io.w) : io.kept ? kept.w : b.w;
   const long long wplane = p.w_direct ? 0 : (long long)s.V * p.Dp;
   for (int k = 0; k < p.pieces; ++k) {
     const int v0 = k * p.piece, V = s.V - v0 < p.piece ? s.V - v0 : p.piece;

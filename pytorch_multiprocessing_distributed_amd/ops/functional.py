@@ -1745,9 +1745,9 @@ def linear_cross_entropy(x, lin, target, ignore_index=-100, compute_dtype=None):
     """``(loss, correct)`` of the classifier ``lin`` on features ``x``: the mean softmax cross-entropy of
     ``x lin.weight^T + lin.bias`` and the top-1 count (int64 [1], on the device) -- what
     :func:`linear`, :func:`cross_entropy` and :func:`correct_count` give, without the [N, V] logits and
-    their fp32 copies.  On a GPU a call with gradients keeps N x V exponentials in the products' width, up to
-    4 GiB; past that it keeps none, and the backward computes the logits again, a piece of the classes at a
-    time.
+    their fp32 copies.  On a GPU a call with gradients keeps N x V exponentials in the products' width (and
+    the weight's copy in it, if it is not read in place), up to 4 GiB; past that it keeps none, and the
+    backward computes the logits again, a piece of the classes at a time.
 
     ``x`` [..., D] and ``target`` [...] (int64 class indices); rows whose target is ``ignore_index`` count
     for nothing, whatever they hold, and get a zero gradient; when no row is left the loss is 0.  A
