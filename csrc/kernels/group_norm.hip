@@ -401,8 +401,10 @@ __global__ __launch_bounds__(1024) void gn_dparam_kernel(const S* __restrict__ s
   const int j = blockIdx.x * 64 + c;
   const long long per = (rows + gridDim.y - 1) / gridDim.y, lo = blockIdx.y * per, hi = min(rows, lo + per);
   double s = 0.0;
-  if (j < 2 * C)
+  if (j < 2 * C) {
+#pragma unroll 8
     for (long long i = lo + r; i < hi; i += 16) s += src[(size_t)i * 2 * C + j];
+  }
   part[r][c] = s;
   __syncthreads();
   if (r == 0 && j < 2 * C) {
@@ -499,8 +501,8 @@ uintptr_t gn_align(std::initializer_list<const void*> ps) {
 
 namespace {
 
-int gn_shares(long long rows) {  // of dparam's first pass: about 256 rows each
-  const long long n = (rows + 255) / 256;
+int gn_shares(long long rows) {  // of dparam's first pass: about 64 rows each, where two passes pay
+  const long long n = rows <= 512 ? 1 : (rows + 63) / 64;
   return n > 64 ? 64 : (int)n;
 }
 
