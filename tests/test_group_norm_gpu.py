@@ -257,6 +257,24 @@ def test_many_samples(n, c):
     assert ((out[rows].double() - ref).abs() <= 2.0 ** -8 * ref.abs() + 2.0 ** -14).all()
 
 
+@pytest.mark.parametrize("n,hw,c,groups", [(700, 3136, 1024, 32), (720, 3136, 1000, 8)])
+def test_offsets_past_32_bits(n, hw, c, groups):
+    # more than 2^31 elements (4.5 GB): the last sample, in registers and split
+    x = torch.randn(n, hw, c, device="cuda", dtype=torch.bfloat16).requires_grad_(True)
+    gn = torch.nn.GroupNorm(groups, c).cuda()
+    out = OF.group_norm_act(x, gn, act="none")
+    dy = torch.zeros_like(out)
+    dy[-1] = torch.randn(hw, c, device="cuda").to(torch.bfloat16)
+    dx, dw = torch.autograd.grad(out, [x, gn.weight], dy)
+    r = _ref(x.detach()[-1:], None, gn.weight.detach(), gn.bias.detach(), dy[-1:], groups, gn.eps, "none")
+    # values of at most 2^3: half a bf16 step, and fp32 errors far below one
+    assert ((out[-1:].double() - r[0]).abs() <= 2.0 ** -8 * r[0].abs() + 2.0 ** -14).all()
+    assert ((dx[-1:].double() - r[1]).abs() <= 2.0 ** -8 * r[1].abs() + 2.0 ** -14).all()
+    assert not dx[-2].any()
+    # fp32 sums of a few thousand terms
+    assert ((dw.double() - r[2]).abs() <= 512 * U32 * r[8] + 2.0 ** -14 * r[9]).all()
+
+
 @pytest.mark.parametrize("act,with_res", [("relu", True), ("silu", True), ("relu", False)])
 def test_backward_twice_over_a_retained_graph(act, with_res):
     for shape in ((4, (56, 56), 64, 32), (6, (14, 14), 64, 32)):
