@@ -107,13 +107,25 @@ __device__ __forceinline__ float ns_ld(const void* p, long long i, bool f32) {
   return f32 ? static_cast<const float*>(p)[i] : bf2f(static_cast<const bf16_t*>(p)[i]);
 }
 
+// v is pinned to its fp32 rounding: where it is a product, the compiler else rounds the product straight to fp16
+// for one of hi and its use in lo, and twice for the other, and the two differ now and then by a whole fp16 step
 __device__ __forceinline__ void split2(float v, unsigned short& hi, unsigned short& lo) {
+  asm("" : "+v"(v));
   const f16_t h = (f16_t)v, l = (f16_t)(v - (float)h);
   hi = __builtin_bit_cast(unsigned short, h);
   lo = __builtin_bit_cast(unsigned short, l);
 }
 __device__ __forceinline__ float join2(unsigned short hi, unsigned short lo) {
   return (float)__builtin_bit_cast(f16_t, hi) + (float)__builtin_bit_cast(f16_t, lo);
+}
+
+// four neighbours of a matrix in two planes, o a multiple of 4
+__device__ __forceinline__ void put_planes(unsigned short* p, long long plane, long long o, const float (&v)[4]) {
+  unsigned short h[4], l[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) split2(v[e], h[e], l[e]);
+  *reinterpret_cast<uint2*>(p + o) = make_uint2(h[0] | ((uint32_t)h[1] << 16), h[2] | ((uint32_t)h[3] << 16));
+  *reinterpret_cast<uint2*>(p + plane + o) = make_uint2(l[0] | ((uint32_t)l[1] << 16), l[2] | ((uint32_t)l[3] << 16));
 }
 
 // ------------------------------------------------------------- norm, start
@@ -199,6 +211,7 @@ __global__ __launch_bounds__(256) void ns_start_kernel(const NsTable* __restrict
   }
   const bool tall = io.tall;
   const int a = threadIdx.x & 63, b = threadIdx.x >> 6;
+#pragma unroll 8
   for (int i = b; i < 64; i += 4) {  // a: along the source's rows
     const int r = tall ? r0 + a : r0 + i, c = tall ? c0 + i : c0 + a;
     const float v = r < s && c < l ? ns_ld(io.src, tall ? (long long)c * s + r : (long long)r * l + c, f32) : 0.f;
@@ -209,13 +222,13 @@ __global__ __launch_bounds__(256) void ns_start_kernel(const NsTable* __restrict
   const float inv = inv_s;
   unsigned short* x = ws + d.xo;
   const long long plane = (long long)s * lp;
-  for (int i = b; i < 64; i += 4) {
-    const int r = r0 + i, c = c0 + a;
+  const int q = (threadIdx.x & 15) * 4;
+#pragma unroll
+  for (int i = threadIdx.x >> 4; i < 64; i += 16) {
+    const int r = r0 + i, c = c0 + q;
     if (r >= s || c >= lp) continue;
-    unsigned short hi, lo;
-    split2(tile[i][a] * inv, hi, lo);
-    x[(long long)r * lp + c] = hi;
-    x[plane + (long long)r * lp + c] = lo;
+    const float v[4] = {tile[i][q] * inv, tile[i][q + 1] * inv, tile[i][q + 2] * inv, tile[i][q + 3] * inv};
+    put_planes(x, plane, (long long)r * lp + c, v);
   }
 }
 
@@ -236,14 +249,6 @@ __device__ __forceinline__ void tri_of(int t, int& im, int& in) {
   while (r * (r + 1) / 2 > t) --r;
   im = r;
   in = t - r * (r + 1) / 2;
-}
-
-__device__ __forceinline__ void put_planes(unsigned short* p, long long plane, long long o, const float (&v)[4]) {
-  unsigned short h[4], l[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) split2(v[e], h[e], l[e]);
-  *reinterpret_cast<uint2*>(p + o) = make_uint2(h[0] | ((uint32_t)h[1] << 16), h[2] | ((uint32_t)h[3] << 16));
-  *reinterpret_cast<uint2*>(p + plane + o) = make_uint2(l[0] | ((uint32_t)l[1] << 16), l[2] | ((uint32_t)l[3] << 16));
 }
 
 // four neighbours n.. of row m of a symmetric matrix [s][up8(s)] (2 planes), and their mirror images.

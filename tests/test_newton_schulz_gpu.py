@@ -66,6 +66,18 @@ def test_large_tiles(m, n):
     _check(u, OF.newton_schulz(u))
 
 
+@pytest.mark.parametrize("steps", [1, 3])
+@pytest.mark.parametrize("m,n", [(200, 130), (512, 128), (257, 1031), (600, 4608), (3990, 4100)])
+def test_planes_hold_22_bits(m, n, steps):
+    """X <- X leaves the normalised matrix: what the two planes hold, entry by entry."""
+    u = _mat(m, n, seed=9)
+    out = OF.newton_schulz(u, steps=steps, coeffs=(1.0, 0.0, 0.0))
+    ref = u.double() / (u.double().norm() + 1e-7)
+    # a split leaves half a step of the lower plane, 2^-22 of the entry (2^-40 where that plane is subnormal), at
+    # the start and after every step but the last; a handful of fp32 operations around each
+    assert ((out.double() - ref).abs() <= steps * (2.0 ** -22 + 6 * 2.0 ** -24) * ref.abs() + steps * 2.0 ** -39).all()
+
+
 def test_a_models_matrices_in_one_call():
     shapes = [(64, 27)] + [(64, 576), (256, 64), (128, 1152), (30, 7), (5, 300)] * 11 + [(512, 512)]
     us = [_mat(m, n, seed=i) for i, (m, n) in enumerate(shapes)]     # more than one group
